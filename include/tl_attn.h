@@ -314,6 +314,23 @@ int tl_rms_norm(void* out, const void* x, const void* weight, int32_t num_tokens
 int tl_fused_add_rms_norm(void* out, void* residual, const void* x, const void* weight, int32_t num_tokens,
                           int32_t hidden_size, float eps, int32_t dtype, void* stream);
 
+/* No counterpart in the reference, whose norm writes 2 bytes that
+ * per_token_fp8_quant_kernel (fp8_gemm.cu:80-93) reads again.  tl_rms_norm
+ * and tl_fused_add_rms_norm with the output as FP8 E4M3 codes under scales
+ * (value = code * scale): with y the norm's fp32 result, not rounded to dtype,
+ *   scale = max|y| / 448,  out = e4m3(y / scale), round to nearest even,
+ * the maximum over the row (group_size 0; scales fp32 [num_tokens]) or over
+ * each group of 32, 64, 128 or 256 channels (scales [num_tokens, hidden_size /
+ * group_size]; hidden_size a multiple of it).  A row or group whose maximum
+ * is below 448 x 2^-126 is kept as zeros under scale 0; one with an infinity
+ * or a NaN gets the scale NaN.  out may not overlap the other tensors; x,
+ * residual and weight aligned to their elements. */
+int tl_rms_norm_fp8(uint8_t* out, float* scales, const void* x, const void* weight, int32_t num_tokens,
+                    int32_t hidden_size, int32_t group_size, float eps, int32_t dtype, void* stream);
+int tl_fused_add_rms_norm_fp8(uint8_t* out, float* scales, void* residual, const void* x, const void* weight,
+                              int32_t num_tokens, int32_t hidden_size, int32_t group_size, float eps, int32_t dtype,
+                              void* stream);
+
 /* Replaces layer_norm (layernorm_kernels.cu:191-211, kernel :102-139):
  * out = (x - mean) * (1 / sqrt(var + eps)) * weight + bias, var the mean of
  * (x - mean)^2 (two passes over the row). */

@@ -530,6 +530,37 @@ int tl_fused_add_rms_norm(void* out, void* residual, const void* x, const void* 
   return ok();
 }
 
+// The norms with an FP8 output (residual: null without the add).
+static int norm_fp8(uint8_t* out, float* scales, void* residual, const void* x, const void* weight, int32_t num_tokens,
+                    int32_t hidden_size, int32_t group_size, float eps, int32_t dtype, void* stream) {
+  const int rc = check_norm(out, x, weight, num_tokens, hidden_size, dtype);
+  if (rc) return rc;
+  if (group_size != 0 && group_size != 32 && group_size != 64 && group_size != 128 && group_size != 256)
+    return fail(TL_ERR_NOT_IMPLEMENTED, "group_size=%d (built: 0, 32, 64, 128, 256)", group_size);
+  if (group_size && hidden_size % group_size)
+    return fail(TL_ERR_INVALID_ARGUMENT, "hidden_size=%d is not a multiple of group_size=%d", hidden_size, group_size);
+  if (num_tokens == 0) return ok();
+  if (!scales) return fail(TL_ERR_INVALID_ARGUMENT, "NULL scales");
+  const uintptr_t el = dtype == TL_DTYPE_F32 ? 3 : 1;
+  if (((uintptr_t)scales & 3) || (((uintptr_t)x | (uintptr_t)weight | (uintptr_t)residual) & el))
+    return fail(TL_ERR_INVALID_ARGUMENT, "scales, x, residual and weight must be aligned to their elements");
+  const tl::NormFp8 a = {out, scales, residual, x, weight, num_tokens, hidden_size, group_size, dtype, eps};
+  if (tl::launch_rms_norm_fp8(a, (hipStream_t)stream)) return fail(TL_ERR_BACKEND, "rms_norm_fp8 launch failed");
+  return ok();
+}
+
+int tl_rms_norm_fp8(uint8_t* out, float* scales, const void* x, const void* weight, int32_t num_tokens,
+                    int32_t hidden_size, int32_t group_size, float eps, int32_t dtype, void* stream) {
+  return norm_fp8(out, scales, nullptr, x, weight, num_tokens, hidden_size, group_size, eps, dtype, stream);
+}
+
+int tl_fused_add_rms_norm_fp8(uint8_t* out, float* scales, void* residual, const void* x, const void* weight,
+                              int32_t num_tokens, int32_t hidden_size, int32_t group_size, float eps, int32_t dtype,
+                              void* stream) {
+  if (num_tokens > 0 && !residual) return fail(TL_ERR_INVALID_ARGUMENT, "NULL residual");
+  return norm_fp8(out, scales, residual, x, weight, num_tokens, hidden_size, group_size, eps, dtype, stream);
+}
+
 int tl_layer_norm(void* out, const void* x, const void* weight, const void* bias, int32_t num_tokens,
                   int32_t hidden_size, float eps, int32_t dtype, void* stream) {
   int rc = check_norm(out, x, weight, num_tokens, hidden_size, dtype);

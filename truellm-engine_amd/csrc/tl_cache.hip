@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "tl_device.hpp"
+#include "tl_fp8.hpp"
 #include "tl_internal.hpp"
 
 namespace tl {
@@ -195,14 +196,6 @@ __global__ __launch_bounds__(256) void reshape_fp8_kernel(
 // * scale), RNE with saturation to +-448 (NaN stays NaN).  VEC: 16 elements
 // per thread with 16-byte loads and one 16-byte store (both buffers 16-byte
 // aligned); otherwise element by element.
-__device__ __forceinline__ float fp8_sat(float v) {
-  const float c = __builtin_fminf(__builtin_fmaxf(v, -448.0f), 448.0f);
-  return (v != v) ? v : c;
-}
-__device__ __forceinline__ uint32_t pack4_fp8(float a, float b, float c, float d) {
-  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_sat(a), fp8_sat(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_sat(c), fp8_sat(d), (int)w, true);
-}
 template <Kind SRC>
 __device__ __forceinline__ float load_elem(const void* p, int64_t i) {
   if constexpr (SRC == Kind::F32) return reinterpret_cast<const float*>(p)[i];

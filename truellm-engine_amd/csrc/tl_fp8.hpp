@@ -1,0 +1,59 @@
+// tl_fp8.hpp -- fp32 values to E4M3 codes, and the scale of a row of them.
+#pragma once
+
+#include <type_traits>
+
+#include "tl_device.hpp"
+
+namespace tl {
+
+__device__ __forceinline__ float fp8_sat(float v) {
+  const float c = __builtin_fminf(__builtin_fmaxf(v, -448.0f), 448.0f);
+  return (v != v) ? v : c;
+}
+__device__ __forceinline__ uint32_t pack4_fp8(float a, float b, float c, float d) {
+  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_sat(a), fp8_sat(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_sat(c), fp8_sat(d), (int)w, true);
+}
+
+// The scale of a row or group whose largest magnitude is amax (its bits:
+// magnitudes order as unsigned integers, infinities and NaN last), and what
+// its elements are multiplied by before they are rounded.  scale = amax / 448
+// (fp8_gemm.cu:80-84).  A row without a scale that fp32 holds as a normal
+// number (all zeros, or below 448 x 2^-126) is kept as zeros under scale 0; a
+// row with an infinity or a NaN has the scale NaN, under which every code
+// reads as NaN.
+struct Fp8Scale {
+  float scale, inv;
+};
+__device__ __forceinline__ Fp8Scale fp8_scale_of(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return {__builtin_bit_cast(float, 0x7fc00000u), __builtin_bit_cast(float, 0x7fc00000u)};
+  const float s = __builtin_bit_cast(float, amax_bits) / 448.0f;
+  return s >= 1.17549435e-38f ? Fp8Scale{s, 1.0f / s} : Fp8Scale{0.f, 0.f};
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// Max over the 2, 4, .. 64 lanes around a lane (aligned groups of LANES).
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_umax(uint32_t v) {
+  static_assert(LANES >= 1 && LANES <= 64 && (LANES & (LANES - 1)) == 0, "a power of two");
+  auto step = [](uint32_t x, auto ctrl) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, false);
+    return x > y ? x : y;
+  };
+  if constexpr (LANES >= 2) v = step(v, std::integral_constant<int, kDppXor1>());
+  if constexpr (LANES >= 4) v = step(v, std::integral_constant<int, kDppXor2>());
+  if constexpr (LANES >= 8) v = step(v, std::integral_constant<int, kDppHalfMirror>());
+  if constexpr (LANES >= 16) v = step(v, std::integral_constant<int, kDppMirror>());
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] > r[1] ? r[0] : r[1];
+  }
+  if constexpr (LANES >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = r[0] > r[1] ? r[0] : r[1];
+  }
+  return v;
+}
+
+}  // namespace tl

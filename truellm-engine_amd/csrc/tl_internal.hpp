@@ -89,6 +89,18 @@ int launch_rms_norm(void* out, void* residual, const void* x, const void* w, int
                     int dtype, hipStream_t stream);
 int launch_layer_norm(void* out, const void* x, const void* w, const void* b, int rows, int hidden, float eps,
                       int dtype, hipStream_t stream);
+// RMSNorm (residual == nullptr) or residual add + RMSNorm with E4M3 codes
+// and scales, one per row (group 0) or per `group` channels.
+struct NormFp8 {
+  uint8_t* out;                 // [rows, hidden]
+  float* scales;                // [rows] or [rows, hidden / group]
+  void* residual;
+  const void* x; const void* weight;
+  int64_t rows;
+  int hidden, group, dtype;
+  float eps;
+};
+int launch_rms_norm_fp8(const NormFp8& a, hipStream_t stream);
 int launch_act_and_mul(void* out, const void* gate, const void* up, int64_t n, int act, int dtype,
                        hipStream_t stream);
 

@@ -21,26 +21,11 @@
 // element per thread.  All of them are HBM-bound at serving sizes.
 #include "tl_device.hpp"
 #include "tl_internal.hpp"
+#include "tl_row.hpp"
 
 namespace tl {
 
 namespace {
-
-constexpr int kNormThreads = 256;
-
-// Sum over the workgroup, returned to every thread.
-__device__ __forceinline__ float block_sum(float v, float* s_part) {
-#pragma unroll
-  for (int o = kWave / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
-  const int wave = threadIdx.x / kWave;
-  __syncthreads();                                   // s_part free from a previous use
-  if (threadIdx.x % kWave == 0) s_part[wave] = v;
-  __syncthreads();
-  float t = 0.f;
-#pragma unroll
-  for (int w = 0; w < kNormThreads / kWave; ++w) t += s_part[w];
-  return t;
-}
 
 template <Kind K>
 __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(void* __restrict__ out, void* __restrict__ residual,
@@ -62,31 +47,6 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(void* __restrict
   const void* src = fused_add ? residual : x;
   for (int i = threadIdx.x; i < hidden; i += kNormThreads)
     store_scalar<K>(out, base + i, load_scalar<K>(src, base + i) * inv * load_scalar<K>(w, i));
-}
-
-// Round to the storage type and back (identity for f32).
-template <Kind K> __device__ __forceinline__ float round_to(float v);
-template <> __device__ __forceinline__ float round_to<Kind::F32>(float v) { return v; }
-template <> __device__ __forceinline__ float round_to<Kind::F16>(float v) { return f16_to_f32(f32_to_f16(v)); }
-template <> __device__ __forceinline__ float round_to<Kind::BF16>(float v) { return bf16_to_f32(f32_to_bf16(v)); }
-
-template <Kind K> __device__ __forceinline__ void unpack8(const u32x4& c, float (&f)[8]) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint16_t b = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-    f[j] = K == Kind::F16 ? f16_to_f32(b) : bf16_to_f32(b);
-  }
-}
-template <Kind K> __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint16_t lo = K == Kind::F16 ? f32_to_f16(f[2 * k]) : f32_to_bf16(f[2 * k]);
-    const uint16_t hi = K == Kind::F16 ? f32_to_f16(f[2 * k + 1]) : f32_to_bf16(f[2 * k + 1]);
-    w[k] = (uint32_t)lo | ((uint32_t)hi << 16);
-  }
-  return u32x4{w[0], w[1], w[2], w[3]};
 }
 
 // 2-byte rows of up to C x 2048 elements (C 16-byte chunks per thread),

@@ -127,6 +127,8 @@ _SIG = {
     "tl_rope_reshape_and_cache": (ctypes.c_int, [_P] * 10 + [_I] * 9 + [_P]),
     "tl_rms_norm": (ctypes.c_int, [_P, _P, _P, _I, _I, _F, _I, _P]),
     "tl_fused_add_rms_norm": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, _F, _I, _P]),
+    "tl_rms_norm_fp8": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, _I, _F, _I, _P]),
+    "tl_fused_add_rms_norm_fp8": (ctypes.c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P]),
     "tl_layer_norm": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, _F, _I, _P]),
     "tl_act_and_mul": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _I, _I, _P]),
     "tl_vq_encode": (ctypes.c_int, [_P, _P, _P, _I, _I, _I, _P]),
@@ -246,6 +248,14 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def _on_gpu(*tensors):
+    """Refuses tensors (None aside) that are not on the current device, whose streams and kernels would not reach
+    them."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.get_device() == _torch().cuda.current_device()):
+            raise TLError(ERR_INVALID_ARGUMENT, f"a tensor on {t.device}, not on the current GPU")
+
+
 def _stream(stream=None):
     torch = _torch()
     s = torch.cuda.current_stream() if stream is None else stream
@@ -342,6 +352,38 @@ def rms_norm(out, x, weight, eps, stream=None):
 def fused_add_rms_norm(out, residual, x, weight, eps, stream=None):
     check(lib.tl_fused_add_rms_norm(_ptr(out), _ptr(residual), _ptr(x), _ptr(weight), x.shape[0], x.shape[1], eps,
                                     dtype_code(x), _stream(stream)))
+
+
+def _norm_fp8_sizes(out, scales, x, weight, group_size, residual=None):
+    """(T, H) of an FP8 norm's tensors, whose sizes the library cannot see."""
+    T, H = x.shape
+    want = (T, H // group_size) if group_size > 0 else (T,)
+    code = dtype_code(x)
+    if not (x.is_contiguous() and out.is_contiguous() and scales.is_contiguous() and out.shape == x.shape
+            and out.element_size() == 1 and tuple(scales.shape) == want and scales.element_size() == 4
+            and weight.numel() == H and weight.dtype == x.dtype and weight.is_contiguous()):
+        raise TLError(ERR_INVALID_ARGUMENT, f"x {tuple(x.shape)} {x.dtype}: out {tuple(out.shape)} {out.dtype}, "
+                      f"scales {tuple(scales.shape)} (fp32 {want}), weight {tuple(weight.shape)} {weight.dtype}")
+    if residual is not None and not (residual.shape == x.shape and residual.dtype == x.dtype
+                                     and residual.is_contiguous()):
+        raise TLError(ERR_INVALID_ARGUMENT, f"residual {tuple(residual.shape)} {residual.dtype}")
+    _on_gpu(out, scales, x, weight, residual)
+    return T, H, code
+
+
+def rms_norm_fp8(out, scales, x, weight, eps, group_size=0, stream=None):
+    """RMSNorm of x [T, H] as E4M3 codes out (uint8 [T, H]) under fp32 scales: [T] (group_size 0) or
+    [T, H / group_size]; value = code * scale."""
+    T, H, code = _norm_fp8_sizes(out, scales, x, weight, group_size)
+    check(lib.tl_rms_norm_fp8(_ptr(out), _ptr(scales), _ptr(x), _ptr(weight), T, H, group_size, eps, code,
+                              _stream(stream)))
+
+
+def fused_add_rms_norm_fp8(out, scales, residual, x, weight, eps, group_size=0, stream=None):
+    """rms_norm_fp8 of residual + x, which replaces residual (in its dtype)."""
+    T, H, code = _norm_fp8_sizes(out, scales, x, weight, group_size, residual)
+    check(lib.tl_fused_add_rms_norm_fp8(_ptr(out), _ptr(scales), _ptr(residual), _ptr(x), _ptr(weight), T, H,
+                                        group_size, eps, code, _stream(stream)))
 
 
 def layer_norm(out, x, weight, bias, eps, stream=None):
