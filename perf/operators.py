@@ -10,6 +10,7 @@ Where `own` is false, run() computes them in elementary torch operations in 32
 bits, rounded once; where it is true, it calls tl_attn.  Codes come back as
 float8 tensors, next to the scales that they are held under.
 """
+import functools
 import math
 import os
 import random
@@ -26,10 +27,10 @@ ROPE_BASE = 10000.0
 ADJACENT, HALVES = 0, 1
 
 
+@functools.cache
 def lib():
-    at = os.path.join(os.getcwd(), "truellm-engine_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
+    """The framework's binding, imported once."""
+    sys.path.insert(0, os.path.join(os.getcwd(), "truellm-engine_amd"))
     import tl_attn
     return tl_attn
 
