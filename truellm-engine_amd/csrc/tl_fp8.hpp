@@ -1,8 +1,6 @@
 // tl_fp8.hpp -- fp32 values to E4M3 codes, and the scale of a row of them.
 #pragma once
 
-#include <type_traits>
-
 #include "tl_device.hpp"
 
 namespace tl {
@@ -33,26 +31,29 @@ __device__ __forceinline__ Fp8Scale fp8_scale_of(uint32_t amax_bits) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// Max over the 2, 4, .. 64 lanes around a lane (aligned groups of LANES).
+// A lane's bits of another lane of its row of 16 (a DPP control of tl_device.hpp).
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_bits(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t lanes_umax_16(uint32_t v) {   // with lane ^ 16
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ uint32_t lanes_umax_32(uint32_t v) {   // with lane ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+// Max over the aligned group of LANES lanes that a lane is in.
 template <int LANES>
 __device__ __forceinline__ uint32_t lanes_umax(uint32_t v) {
   static_assert(LANES >= 1 && LANES <= 64 && (LANES & (LANES - 1)) == 0, "a power of two");
-  auto step = [](uint32_t x, auto ctrl) {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, false);
-    return x > y ? x : y;
-  };
-  if constexpr (LANES >= 2) v = step(v, std::integral_constant<int, kDppXor1>());
-  if constexpr (LANES >= 4) v = step(v, std::integral_constant<int, kDppXor2>());
-  if constexpr (LANES >= 8) v = step(v, std::integral_constant<int, kDppHalfMirror>());
-  if constexpr (LANES >= 16) v = step(v, std::integral_constant<int, kDppMirror>());
-  if constexpr (LANES >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = r[0] > r[1] ? r[0] : r[1];
-  }
-  if constexpr (LANES >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = r[0] > r[1] ? r[0] : r[1];
-  }
+  if constexpr (LANES >= 2) v = max(v, lane_bits<kDppXor1>(v));
+  if constexpr (LANES >= 4) v = max(v, lane_bits<kDppXor2>(v));
+  if constexpr (LANES >= 8) v = max(v, lane_bits<kDppHalfMirror>(v));
+  if constexpr (LANES >= 16) v = max(v, lane_bits<kDppMirror>(v));
+  if constexpr (LANES >= 32) v = lanes_umax_16(v);
+  if constexpr (LANES >= 64) v = lanes_umax_32(v);
   return v;
 }
 

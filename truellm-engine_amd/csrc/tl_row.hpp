@@ -22,6 +22,13 @@ __device__ __forceinline__ float block_sum(float v, float* s_part) {
   return t;
 }
 
+// Sum over the wavefront, returned to every lane.
+__device__ __forceinline__ float wave_total(float v) {
+  v = row_sum(v);
+  v = swap16_add(v, v);
+  return swap32_add(v, v);
+}
+
 // Round to the storage type and back (identity for f32).
 template <Kind K> __device__ __forceinline__ float round_to(float v);
 template <> __device__ __forceinline__ float round_to<Kind::F32>(float v) { return v; }
