@@ -270,6 +270,67 @@ int tl_rope_reshape_and_cache(const void* q, void* q_out, const void* key, const
                               int32_t num_kv_heads, int32_t head_size, int32_t block_size,
                               int32_t num_blocks, int32_t dtype, int32_t style, void* stream);
 
+/* No counterpart in the reference.  FP8 pools that need no calibration: each
+ * row (one token of one kv head) has a scale of its own, found as the row is
+ * written,
+ *   scale = max|row| / 448,  code = e4m3(row / scale),  value = code * scale,
+ * in k_scales / v_scales fp32 [N, n_kv, block_size] beside the pools
+ * [N, n_kv, head_size, block_size].  A row whose maximum is below 448 x
+ * 2^-126 is kept as zeros under scale 0; a row with an infinity or a NaN gets
+ * the scale NaN and reads as NaN.  tl_copy_blocks and tl_swap_blocks move
+ * the scales as they move pools (block_bytes n_kv * block_size * 4).
+ * tl_reshape_and_cache_fp8 with such scales: key / value [T, n_kv,
+ * head_size] of src_dtype F16 or BF16, head_size 128, any block_size; slots
+ * as there (< 0 or past the pool: nothing written), none twice in a call.
+ * Calls of few tokens rewrite the bytes around a token's slot (up to its
+ * block's rows of a kv head, the other slots with their own bytes), so a
+ * block that the call writes to has no other writer during it. */
+int tl_reshape_and_cache_fp8_scaled(const void* key, const void* value, int32_t src_dtype, uint8_t* k_cache,
+                                    uint8_t* v_cache, float* k_scales, float* v_scales,
+                                    const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                                    int32_t head_size, int32_t block_size, int32_t num_blocks, void* stream);
+
+/* No counterpart in the reference.  tl_rope_reshape_and_cache for positions
+ * with several axes (time, height, width of image and video tokens): pair i
+ * of a head is turned by the tables' row of its token's position on one axis,
+ *   c, s = tables[positions[axis(i)][t]][i],
+ * with the rotation given there; one axis is that call's.  axis_pairs[a]
+ * pairs belong to axis a (their sum is head_size / 2): consecutive runs of
+ * pairs, or with `interleaved` dealt out in turn, an axis without pairs left
+ * being passed over. */
+#define TL_ROPE_MAX_AXES 4
+typedef struct tl_rope_axes_desc {
+  int32_t num_heads;           /* q heads; 0: key / value only */
+  int32_t num_kv_heads;
+  int32_t head_size;           /* a multiple of 16, at most 256; 128 with an FP8 pool */
+  int32_t block_size;
+  int32_t num_blocks;
+  int32_t dtype;               /* q, q_out, key, value: F16, BF16 or F32 */
+  int32_t kv_dtype;            /* the pools: dtype, or FP8_E4M3 with scales (dtype F16 or BF16) */
+  int32_t style;               /* tl_rope_style */
+  int32_t num_axes;            /* 1 .. TL_ROPE_MAX_AXES */
+  int32_t axis_pairs[TL_ROPE_MAX_AXES];
+  int32_t interleaved;
+  int32_t max_positions;       /* rows of the tables */
+} tl_rope_axes_desc;
+
+/* q [T, num_heads, d] -> q_out (may be q), key / value [T, n_kv, d] into the
+ * pools; k_scales / v_scales as above for FP8 pools (of the rotated key,
+ * which is not rounded to dtype first), NULL otherwise.  positions int32
+ * [num_axes, T]; a token with a position outside [0, max_positions) on some
+ * axis is not written at all.  The strides are the elements from a token to
+ * the next of q, q_out, key and value (0: the heads' own size), so that
+ * slices of one projection's output can be passed; a head's elements and a
+ * token's heads are contiguous.  Slots as for
+ * tl_reshape_and_cache_fp8_scaled; calls of few tokens rewrite bytes around
+ * their slots as that call does, into pools of either type. */
+int tl_rope_axes_reshape_and_cache(const tl_rope_axes_desc* desc, const void* q, void* q_out, const void* key,
+                                   const void* value, void* k_cache, void* v_cache, float* k_scales,
+                                   float* v_scales, const int32_t* slot_mapping, const int32_t* positions,
+                                   const float* cos_table, const float* sin_table, int32_t num_tokens,
+                                   int32_t q_stride, int32_t q_out_stride, int32_t key_stride,
+                                   int32_t value_stride, void* stream);
+
 /* ------------------------------------------------------------------------
  * KV-cache block management
  * --------------------------------------------------------------------- */

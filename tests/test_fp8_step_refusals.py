@@ -55,3 +55,113 @@ def test_norm_fp8_binding_refuses_wrong_tensors():
         if "res" not in kw:
             with pytest.raises(tla.TLError):
                 tla.rms_norm_fp8(a["out"], a["s"], a["x"], a["w"], 1e-5, a["group"])
+
+
+def _axes_desc(**kw):
+    d = tla.RopeAxesDesc()
+    d.num_heads, d.num_kv_heads, d.head_size, d.block_size, d.num_blocks = 8, 2, 128, 16, 64
+    d.dtype = d.kv_dtype = tla.BF16
+    d.style, d.num_axes, d.interleaved, d.max_positions = tla.ROPE_HALVES, 3, 0, 4096
+    d.axis_pairs[0], d.axis_pairs[1], d.axis_pairs[2] = 16, 24, 24
+    for k, v in kw.items():
+        if k == "axis_pairs":
+            for i in range(4):
+                d.axis_pairs[i] = v[i] if i < len(v) else 0
+        else:
+            setattr(d, k, v)
+    return d
+
+
+def _axes(d, T=4, q=FAKE, q_out=FAKE, key=FAKE, value=FAKE, k=FAKE, v=FAKE, ks=None, vs=None, slots=FAKE, pos=FAKE,
+          cos=FAKE, sin=FAKE, strides=(0, 0, 0, 0)):
+    return L.tl_rope_axes_reshape_and_cache(None if d is None else ctypes.byref(d), q, q_out, key, value, k, v, ks, vs,
+                                            slots, pos, cos, sin, T, *strides, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(num_kv_heads=0), tla.ERR_INVALID_ARGUMENT), (dict(num_heads=-1), tla.ERR_INVALID_ARGUMENT),
+    (dict(head_size=120), tla.ERR_INVALID_ARGUMENT), (dict(head_size=272, axis_pairs=[136]), tla.ERR_NOT_IMPLEMENTED),
+    (dict(block_size=0), tla.ERR_INVALID_ARGUMENT), (dict(num_blocks=0), tla.ERR_INVALID_ARGUMENT),
+    (dict(max_positions=0), tla.ERR_INVALID_ARGUMENT), (dict(dtype=9), tla.ERR_INVALID_ARGUMENT),
+    (dict(dtype=tla.FP8_E4M3, kv_dtype=tla.FP8_E4M3), tla.ERR_INVALID_ARGUMENT),
+    (dict(kv_dtype=tla.F16), tla.ERR_NOT_IMPLEMENTED),
+    (dict(dtype=tla.F32, kv_dtype=tla.FP8_E4M3), tla.ERR_NOT_IMPLEMENTED),
+    (dict(style=2), tla.ERR_INVALID_ARGUMENT), (dict(interleaved=2), tla.ERR_INVALID_ARGUMENT),
+    (dict(num_axes=0), tla.ERR_INVALID_ARGUMENT), (dict(num_axes=5), tla.ERR_INVALID_ARGUMENT),
+    (dict(axis_pairs=[16, 24, 23]), tla.ERR_INVALID_ARGUMENT), (dict(axis_pairs=[16, 25, 24]), tla.ERR_INVALID_ARGUMENT),
+    (dict(axis_pairs=[-1, 41, 24]), tla.ERR_INVALID_ARGUMENT),
+    (dict(axis_pairs=[16, 24, 0, 24]), tla.ERR_INVALID_ARGUMENT),      # the fourth is not one of num_axes
+    (dict(axis_pairs=[2**31 - 1, 2**31 - 1, 66]), tla.ERR_INVALID_ARGUMENT),
+    (dict(num_blocks=2**27, block_size=32), tla.ERR_INVALID_ARGUMENT)])
+def test_rope_axes_refuses_descriptors(kw, code):
+    assert _axes(_axes_desc(**kw)) == code
+    assert tla.last_error()
+
+
+def test_rope_axes_refuses_arguments():
+    assert _axes(None) == tla.ERR_INVALID_ARGUMENT
+    d, f = _axes_desc(), _axes_desc(kv_dtype=tla.FP8_E4M3)
+    assert _axes(d, T=-1) == tla.ERR_INVALID_ARGUMENT
+    for name in ("q", "q_out", "key", "value", "k", "v", "slots", "pos", "cos", "sin"):
+        assert _axes(d, **{name: None}) == tla.ERR_INVALID_ARGUMENT, name
+    for name in ("q", "q_out", "key", "value", "k", "v"):
+        assert _axes(d, **{name: ODD}) == tla.ERR_INVALID_ARGUMENT, name
+    assert _axes(d, ks=FAKE, vs=FAKE) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(f) == tla.ERR_INVALID_ARGUMENT                        # no scales
+    assert _axes(f, ks=FAKE) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(f, ks=FAKE, vs=ctypes.c_void_p(0x1002)) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(_axes_desc(kv_dtype=tla.FP8_E4M3, head_size=64, axis_pairs=[8, 12, 12]), ks=FAKE, vs=FAKE) \
+        == tla.ERR_NOT_IMPLEMENTED
+    for i, row in enumerate((8 * 128, 8 * 128, 2 * 128, 2 * 128)):
+        s = [0, 0, 0, 0]
+        s[i] = row - 1
+        assert _axes(d, strides=s) == tla.ERR_INVALID_ARGUMENT
+        s[i] = -row
+        assert _axes(d, strides=s) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(d, T=0, q=None, q_out=None, key=None, value=None, k=None, v=None, slots=None, pos=None, cos=None,
+                 sin=None) == tla.OK
+
+
+def test_fp8_scaled_append_refuses():
+    def call(T=4, n_kv=2, D=128, BS=16, N=64, dtype=tla.F16, key=FAKE, value=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE,
+             slots=FAKE):
+        return L.tl_reshape_and_cache_fp8_scaled(key, value, dtype, k, v, ks, vs, slots, T, n_kv, D, BS, N, None)
+    for kw in (dict(T=-1), dict(n_kv=0), dict(D=0), dict(BS=0), dict(N=0), dict(key=None), dict(value=None), dict(k=None),
+               dict(v=None), dict(ks=None), dict(vs=None), dict(slots=None), dict(key=ODD), dict(value=ODD),
+               dict(ks=ctypes.c_void_p(0x1002)), dict(N=2**28, BS=16)):
+        assert call(**kw) == tla.ERR_INVALID_ARGUMENT, kw
+    for kw in (dict(dtype=tla.F32), dict(dtype=tla.FP8_E4M3), dict(D=64), dict(D=256)):
+        assert call(**kw) == tla.ERR_NOT_IMPLEMENTED, kw
+    assert call(T=0, key=None, value=None, k=None, v=None, ks=None, vs=None, slots=None) == tla.OK
+
+
+def test_append_bindings_refuse_wrong_tensors():
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    good = dict(q=torch.zeros(4, 8, 128, dtype=bf), key=torch.zeros(4, 2, 128, dtype=bf),
+                value=torch.zeros(4, 2, 128, dtype=bf), k=torch.zeros(6, 2, 128, 16, dtype=u8),
+                v=torch.zeros(6, 2, 128, 16, dtype=u8), slots=torch.zeros(4, dtype=i32),
+                pos=torch.zeros(3, 4, dtype=i32), cos=torch.zeros(99, 64), sin=torch.zeros(99, 64),
+                q_out=torch.zeros(4, 8, 128, dtype=bf), ks=torch.zeros(6, 2, 16), vs=torch.zeros(6, 2, 16))
+    desc = tla.make_rope_axes_desc(good["q"], good["key"], good["k"], [16, 24, 24], 99)
+
+    def call(**kw):
+        a = {**good, **kw}
+        tla.rope_axes_reshape_and_cache(desc, a["q"], a["key"], a["value"], a["k"], a["v"], a["slots"], a["pos"],
+                                        a["cos"], a["sin"], q_out=a["q_out"], k_scales=a["ks"], v_scales=a["vs"])
+    for kw in (dict(q=good["q"][:3]), dict(q=good["q"].half()), dict(q_out=good["q"][:, :4]), dict(key=good["key"][:3]),
+               dict(key=good["key"].float()), dict(value=good["value"][:3]), dict(value=good["value"].half()),
+               dict(key=torch.zeros(4, 128, 2, dtype=bf).transpose(1, 2)), dict(q=good["q"][:1].expand(4, 8, 128)),
+               dict(k=good["k"][:5]), dict(v=good["v"].to(bf)), dict(k=good["k"].transpose(0, 1)),
+               dict(slots=good["slots"].long()), dict(slots=good["slots"][:3]), dict(pos=good["pos"][:2]),
+               dict(pos=torch.zeros(4, 3, dtype=i32).t()), dict(cos=good["cos"][:98]), dict(sin=good["sin"].double()),
+               dict(ks=good["ks"][:5]), dict(vs=good["vs"].half()), dict()):      # the last: not on a GPU
+        with pytest.raises(tla.TLError):
+            call(**kw)
+    for bad in ([], [1] * 5):
+        with pytest.raises(tla.TLError):
+            tla.make_rope_axes_desc(good["q"], good["key"], good["k"], bad, 99)
+    for kw in (dict(key=good["key"][:3]), dict(value=good["value"].half()), dict(ks=good["ks"].half()),
+               dict(k=good["k"].to(bf), v=good["v"].to(bf)), dict(slots=good["slots"].long()), dict()):
+        a = {**good, **kw}
+        with pytest.raises(tla.TLError):
+            tla.reshape_and_cache_fp8_scaled(a["key"], a["value"], a["k"], a["v"], a["ks"], a["vs"], a["slots"])

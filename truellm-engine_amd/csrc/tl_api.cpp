@@ -503,6 +503,131 @@ int tl_rope_reshape_and_cache(const void* q, void* q_out, const void* key, const
   return ok();
 }
 
+// What FP8 pools with a scale for each token and head need.
+static int check_scales(const float* k_scales, const float* v_scales, int32_t head_size) {
+  if (head_size != 128) return fail(TL_ERR_NOT_IMPLEMENTED, "scaled FP8 pools: head_size=%d (built: 128)", head_size);
+  if (!k_scales || !v_scales) return fail(TL_ERR_INVALID_ARGUMENT, "FP8 pools need k_scales and v_scales");
+  if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3)
+    return fail(TL_ERR_INVALID_ARGUMENT, "k_scales / v_scales misaligned");
+  return TL_OK;
+}
+
+// Slots are int32: a pool past 2^31 of them has blocks that none can name.
+static int check_slots(int32_t num_blocks, int32_t block_size) {
+  if ((int64_t)num_blocks * block_size > ((int64_t)1 << 31))
+    return fail(TL_ERR_INVALID_ARGUMENT, "num_blocks=%d x block_size=%d slots exceed int32", num_blocks, block_size);
+  return TL_OK;
+}
+
+int tl_reshape_and_cache_fp8_scaled(const void* key, const void* value, int32_t src_dtype, uint8_t* k_cache,
+                                    uint8_t* v_cache, float* k_scales, float* v_scales,
+                                    const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                                    int32_t head_size, int32_t block_size, int32_t num_blocks, void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0 || head_size <= 0 || block_size <= 0 || num_blocks <= 0)
+    return fail(TL_ERR_INVALID_ARGUMENT, "num_tokens=%d num_kv_heads=%d head_size=%d block_size=%d num_blocks=%d",
+                num_tokens, num_kv_heads, head_size, block_size, num_blocks);
+  if (src_dtype != TL_DTYPE_F16 && src_dtype != TL_DTYPE_BF16)
+    return fail(TL_ERR_NOT_IMPLEMENTED, "src_dtype=%d (F16 or BF16 sources)", src_dtype);
+  int rc = check_slots(num_blocks, block_size);
+  if (rc) return rc;
+  if (num_tokens == 0) return ok();
+  rc = check_scales(k_scales, v_scales, head_size);
+  if (rc) return rc;
+  if (!key || !value || !k_cache || !v_cache || !slot_mapping)
+    return fail(TL_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (((uintptr_t)key | (uintptr_t)value) & 1) return fail(TL_ERR_INVALID_ARGUMENT, "key / value misaligned");
+  tl::AxesAppend a;
+  memset(&a, 0, sizeof a);
+  a.key = key; a.value = value; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.k_scales = k_scales; a.v_scales = v_scales; a.slots = slot_mapping;
+  a.num_tokens = num_tokens; a.num_kv_heads = num_kv_heads; a.head_size = head_size;
+  a.block_size = block_size; a.num_blocks = num_blocks;
+  a.dtype = src_dtype; a.kv_dtype = TL_DTYPE_FP8_E4M3;
+  a.key_stride = a.value_stride = (int64_t)num_kv_heads * head_size;
+  if (tl::launch_axes_append(a, (hipStream_t)stream))
+    return fail(TL_ERR_BACKEND, "reshape_and_cache_fp8_scaled launch failed");
+  return ok();
+}
+
+int tl_rope_axes_reshape_and_cache(const tl_rope_axes_desc* d, const void* q, void* q_out, const void* key,
+                                   const void* value, void* k_cache, void* v_cache, float* k_scales,
+                                   float* v_scales, const int32_t* slot_mapping, const int32_t* positions,
+                                   const float* cos_table, const float* sin_table, int32_t num_tokens,
+                                   int32_t q_stride, int32_t q_out_stride, int32_t key_stride,
+                                   int32_t value_stride, void* stream) {
+  if (!d) return fail(TL_ERR_INVALID_ARGUMENT, "desc is NULL");
+  if (num_tokens < 0 || d->num_heads < 0 || d->num_kv_heads <= 0 || d->head_size <= 0 || d->block_size <= 0 ||
+      d->num_blocks <= 0 || d->max_positions <= 0)
+    return fail(TL_ERR_INVALID_ARGUMENT,
+                "num_tokens=%d num_heads=%d num_kv_heads=%d head_size=%d block_size=%d num_blocks=%d "
+                "max_positions=%d", num_tokens, d->num_heads, d->num_kv_heads, d->head_size, d->block_size,
+                d->num_blocks, d->max_positions);
+  if (d->head_size % 16) return fail(TL_ERR_INVALID_ARGUMENT, "head_size=%d must be a multiple of 16", d->head_size);
+  if (d->head_size > 256) return fail(TL_ERR_NOT_IMPLEMENTED, "head_size=%d (built: up to 256)", d->head_size);
+  if (!is_float_kind(d->dtype)) return fail(TL_ERR_INVALID_ARGUMENT, "dtype=%d", d->dtype);
+  if (d->style != TL_ROPE_ADJACENT && d->style != TL_ROPE_HALVES)
+    return fail(TL_ERR_INVALID_ARGUMENT, "style=%d", d->style);
+  if (d->interleaved != 0 && d->interleaved != 1) return fail(TL_ERR_INVALID_ARGUMENT, "interleaved=%d", d->interleaved);
+  const bool fp8 = d->kv_dtype == TL_DTYPE_FP8_E4M3;
+  if (!fp8 && d->kv_dtype != d->dtype)
+    return fail(TL_ERR_NOT_IMPLEMENTED, "kv_dtype=%d with dtype=%d (built: the same, or FP8_E4M3)", d->kv_dtype, d->dtype);
+  if (fp8 && d->dtype == TL_DTYPE_F32) return fail(TL_ERR_NOT_IMPLEMENTED, "FP8 pools take F16 or BF16 tensors");
+  if (d->num_axes < 1 || d->num_axes > TL_ROPE_MAX_AXES)
+    return fail(TL_ERR_INVALID_ARGUMENT, "num_axes=%d (1 .. %d)", d->num_axes, TL_ROPE_MAX_AXES);
+  int64_t pairs = 0;
+  for (int x = 0; x < d->num_axes; ++x) {
+    if (d->axis_pairs[x] < 0) return fail(TL_ERR_INVALID_ARGUMENT, "axis_pairs[%d]=%d", x, d->axis_pairs[x]);
+    pairs += d->axis_pairs[x];
+  }
+  if (pairs != d->head_size / 2)
+    return fail(TL_ERR_INVALID_ARGUMENT, "axis_pairs sum to %lld, head_size / 2 is %d", (long long)pairs, d->head_size / 2);
+  const int64_t q_row = (int64_t)d->num_heads * d->head_size, kv_row = (int64_t)d->num_kv_heads * d->head_size;
+  if ((q_stride && q_stride < q_row) || (q_out_stride && q_out_stride < q_row) ||
+      (key_stride && key_stride < kv_row) || (value_stride && value_stride < kv_row))
+    return fail(TL_ERR_INVALID_ARGUMENT, "strides q=%d q_out=%d key=%d value=%d below a token's heads", q_stride,
+                q_out_stride, key_stride, value_stride);
+  int rc = check_slots(d->num_blocks, d->block_size);
+  if (rc) return rc;
+  if (num_tokens == 0) return ok();
+  if (fp8) {
+    rc = check_scales(k_scales, v_scales, d->head_size);
+    if (rc) return rc;
+  } else if (k_scales || v_scales) {
+    return fail(TL_ERR_INVALID_ARGUMENT, "scales with a pool that is not FP8_E4M3");
+  }
+  if (!key || !value || !k_cache || !v_cache || !slot_mapping || !positions || !cos_table || !sin_table ||
+      (d->num_heads > 0 && (!q || !q_out)))
+    return fail(TL_ERR_INVALID_ARGUMENT, "NULL pointer");
+  const uintptr_t el = d->dtype == TL_DTYPE_F32 ? 3 : 1;
+  if (((uintptr_t)key | (uintptr_t)value | (uintptr_t)q | (uintptr_t)q_out) & el ||
+      (!fp8 && ((uintptr_t)k_cache | (uintptr_t)v_cache) & el))
+    return fail(TL_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+  tl::AxesAppend a;
+  memset(&a, 0, sizeof a);
+  a.q = q; a.q_out = q_out; a.key = key; a.value = value; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.k_scales = k_scales; a.v_scales = v_scales; a.slots = slot_mapping; a.positions = positions;
+  a.cos_table = cos_table; a.sin_table = sin_table;
+  a.q_stride = q_stride ? q_stride : q_row;
+  a.q_out_stride = q_out_stride ? q_out_stride : q_row;
+  a.key_stride = key_stride ? key_stride : kv_row;
+  a.value_stride = value_stride ? value_stride : kv_row;
+  a.num_tokens = num_tokens; a.num_heads = d->num_heads; a.num_kv_heads = d->num_kv_heads;
+  a.head_size = d->head_size; a.block_size = d->block_size; a.num_blocks = d->num_blocks;
+  a.max_positions = d->max_positions; a.dtype = d->dtype; a.kv_dtype = d->kv_dtype; a.style = d->style;
+  a.num_axes = d->num_axes;
+  int left[TL_ROPE_MAX_AXES] = {}, axis = 0;
+  for (int x = 0; x < d->num_axes; ++x) left[x] = d->axis_pairs[x];
+  for (int i = 0; i < d->head_size / 2; ++i) {
+    while (left[axis] == 0) axis = (axis + 1) % d->num_axes;   // ends: pairs are left
+    a.axis_of[i / 16] |= (uint32_t)axis << (2 * (i % 16));
+    --left[axis];
+    if (d->interleaved) axis = (axis + 1) % d->num_axes;
+  }
+  if (tl::launch_axes_append(a, (hipStream_t)stream))
+    return fail(TL_ERR_BACKEND, "rope_axes_reshape_and_cache launch failed");
+  return ok();
+}
+
 static int check_norm(const void* out, const void* x, const void* weight, int32_t rows, int32_t hidden,
                       int32_t dtype) {
   if (rows < 0 || hidden <= 0) return fail(TL_ERR_INVALID_ARGUMENT, "num_tokens=%d hidden_size=%d", rows, hidden);

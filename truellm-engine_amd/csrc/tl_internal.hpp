@@ -84,6 +84,24 @@ int launch_rope_cache(const RopeCache& a, hipStream_t stream);
 // RoPE of q (into q_out) and of the keys (into k_out), nothing else written.
 int launch_rope_rows(const RopeCache& a, hipStream_t stream);
 
+// RoPE with a position on each of num_axes axes (0: no rotation), then key
+// and value into pools of their own type, or into FP8 pools with a scale for
+// each token and kv head.
+struct AxesAppend {
+  const void* q; void* q_out;   // [T, H, d], token strides below
+  const void* key; const void* value;   // [T, n_kv, d]
+  void* k_cache; void* v_cache; // [N, n_kv, d, BS]
+  float* k_scales; float* v_scales;     // FP8: [N, n_kv, BS]
+  const int32_t* slots;         // [T]
+  const int32_t* positions;     // [num_axes, T]
+  const float* cos_table; const float* sin_table;   // [max_positions, d/2]
+  int64_t q_stride, q_out_stride, key_stride, value_stride;   // elements from token to token
+  int num_tokens, num_heads, num_kv_heads, head_size, block_size, num_blocks, max_positions;
+  int dtype, kv_dtype, style, num_axes;
+  uint32_t axis_of[8];          // 2 bits for each pair
+};
+int launch_axes_append(const AxesAppend& a, hipStream_t stream);
+
 // Norms and gated activations (residual == nullptr: plain RMSNorm).
 int launch_rms_norm(void* out, void* residual, const void* x, const void* w, int rows, int hidden, float eps,
                     int dtype, hipStream_t stream);

@@ -107,6 +107,27 @@ class PrefillDesc(ctypes.Structure):
         ("v_scale", ctypes.c_float),
     ]
 
+
+ROPE_MAX_AXES = 4
+
+
+class RopeAxesDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("style", ctypes.c_int32),
+        ("num_axes", ctypes.c_int32),
+        ("axis_pairs", ctypes.c_int32 * ROPE_MAX_AXES),
+        ("interleaved", ctypes.c_int32),
+        ("max_positions", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
@@ -125,6 +146,8 @@ _SIG = {
     "tl_reshape_and_cache": (ctypes.c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "tl_reshape_and_cache_fp8": (ctypes.c_int, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P]),
     "tl_rope_reshape_and_cache": (ctypes.c_int, [_P] * 10 + [_I] * 9 + [_P]),
+    "tl_reshape_and_cache_fp8_scaled": (ctypes.c_int, [_P, _P, _I] + [_P] * 5 + [_I] * 5 + [_P]),
+    "tl_rope_axes_reshape_and_cache": (ctypes.c_int, [ctypes.POINTER(RopeAxesDesc)] + [_P] * 12 + [_I] * 5 + [_P]),
     "tl_rms_norm": (ctypes.c_int, [_P, _P, _P, _I, _I, _F, _I, _P]),
     "tl_fused_add_rms_norm": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, _F, _I, _P]),
     "tl_rms_norm_fp8": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, _I, _F, _I, _P]),
@@ -434,6 +457,98 @@ def rope_reshape_and_cache(q, key, value, k_cache, v_cache, slot_mapping, positi
         _ptr(q), _ptr(q_out), _ptr(key), _ptr(value), _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping),
         _ptr(positions), _ptr(cos_table), _ptr(sin_table), cos_table.shape[0], T, H, n_kv, D,
         k_cache.shape[3], k_cache.shape[0], dtype_code(key), style, _stream(stream)))
+
+
+def make_rope_axes_desc(q, key, k_cache, axis_pairs, max_positions, *, style=ROPE_ADJACENT, interleaved=False):
+    """q [T, H, D] or None, key [T, n_kv, D], k_cache [N, n_kv, D, bs] (uint8: FP8 with scales); axis_pairs: the pairs
+    of a head that each axis turns, in consecutive runs or (interleaved) dealt out in turn; max_positions: rows of the
+    tables.  Independent of the number of tokens."""
+    if not 1 <= len(axis_pairs) <= ROPE_MAX_AXES:
+        raise TLError(ERR_INVALID_ARGUMENT, f"{len(axis_pairs)} axes (1 .. {ROPE_MAX_AXES})")
+    d = RopeAxesDesc()
+    d.num_heads = 0 if q is None else q.shape[1]
+    d.num_kv_heads, d.head_size = key.shape[1], key.shape[2]
+    d.block_size, d.num_blocks = k_cache.shape[3], k_cache.shape[0]
+    d.dtype, d.kv_dtype, d.style = dtype_code(key), dtype_code(k_cache), style
+    d.num_axes, d.interleaved, d.max_positions = len(axis_pairs), int(bool(interleaved)), max_positions
+    for i, n in enumerate(axis_pairs):
+        d.axis_pairs[i] = n
+    return d
+
+
+def _token_stride(t, heads, head_size, dtype, what):
+    """Elements from a token of t [T, heads, head_size] to the next; its heads lie together."""
+    T = t.shape[0]
+    if (tuple(t.shape[1:]) != (heads, head_size) or dtype_code(t) != dtype or t.stride(2) != 1
+            or (heads > 1 and t.stride(1) != head_size) or (T > 1 and t.stride(0) < heads * head_size)):
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} strides {t.stride()}: "
+                      f"[T, {heads}, {head_size}] with the heads of a token together")
+    return t.stride(0) if T > 1 else 0
+
+
+def _check_pools(k_cache, v_cache, k_scales, v_scales, num_blocks, heads, head_size, block_size):
+    """Pools [N, n_kv, D, bs] of one type, and their scales (None: none) fp32 [N, n_kv, bs]."""
+    shape = (num_blocks, heads, head_size, block_size)
+    if not (tuple(k_cache.shape) == shape and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
+            and k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise TLError(ERR_INVALID_ARGUMENT, f"pools {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} "
+                      f"{v_cache.dtype}: contiguous {shape} of one type")
+    for s in (k_scales, v_scales):
+        if s is not None and not (tuple(s.shape) == (num_blocks, heads, block_size) and dtype_code(s) == F32
+                                  and s.is_contiguous()):
+            raise TLError(ERR_INVALID_ARGUMENT, f"scales {tuple(s.shape)} {s.dtype}: contiguous fp32 "
+                          f"{(num_blocks, heads, block_size)}")
+
+
+def _check_ints(t, shape, what):
+    if tuple(t.shape) != shape or t.dtype != _torch().int32 or not t.is_contiguous():
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype}: contiguous int32 {shape}")
+
+
+def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_cache, slot_mapping, positions, cos_table,
+                                sin_table, q_out=None, k_scales=None, v_scales=None, stream=None):
+    """RoPE with a position on each axis, positions int32 [axes, T], of q (into q_out, default in place) and key, then
+    key/value into the pools; FP8 pools (uint8) take k_scales / v_scales fp32 [N, n_kv, bs], one scale per token and
+    head.  q, q_out, key and value may be slices of a wider tensor (their token strides are read)."""
+    T, H, n_kv, D = key.shape[0], desc.num_heads, desc.num_kv_heads, desc.head_size
+    q_out = q if q_out is None else q_out
+    strides = [0, 0]
+    if H:
+        strides = [_token_stride(q, H, D, desc.dtype, "q"), _token_stride(q_out, H, D, desc.dtype, "q_out")]
+        if q.shape[0] != T or q_out.shape[0] != T:
+            raise TLError(ERR_INVALID_ARGUMENT, f"q has {q.shape[0]}, q_out {q_out.shape[0]} tokens, key {T}")
+    strides += [_token_stride(key, n_kv, D, desc.dtype, "key"), _token_stride(value, n_kv, D, desc.dtype, "value")]
+    _check_pools(k_cache, v_cache, k_scales, v_scales, desc.num_blocks, n_kv, D, desc.block_size)
+    _check_ints(slot_mapping, (T,), "slot_mapping")
+    _check_ints(positions, (desc.num_axes, T), "positions")
+    table = (desc.max_positions, D // 2)
+    if value.shape[0] != T or dtype_code(k_cache) != desc.kv_dtype or any(
+            tuple(t.shape) != table or dtype_code(t) != F32 or not t.is_contiguous() for t in (cos_table, sin_table)):
+        raise TLError(ERR_INVALID_ARGUMENT, f"value has {value.shape[0]} tokens of {T}, pools {k_cache.dtype}, tables "
+                      f"{tuple(cos_table.shape)}, {tuple(sin_table.shape)} (fp32 {table})")
+    _on_gpu(q if H else None, q_out if H else None, key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping,
+            positions, cos_table, sin_table)
+    check(lib.tl_rope_axes_reshape_and_cache(
+        ctypes.byref(desc), _ptr(q), _ptr(q_out), _ptr(key), _ptr(value), _ptr(k_cache), _ptr(v_cache),
+        _ptr(k_scales), _ptr(v_scales), _ptr(slot_mapping), _ptr(positions), _ptr(cos_table), _ptr(sin_table), T,
+        *strides, _stream(stream)))
+
+
+def reshape_and_cache_fp8_scaled(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, stream=None):
+    """reshape_and_cache_fp8 with a scale for each token and head, found here: k_scales / v_scales fp32
+    [N, n_kv, bs]."""
+    T, n_kv, D = key.shape
+    if not (key.is_contiguous() and value.is_contiguous() and value.shape == key.shape and value.dtype == key.dtype):
+        raise TLError(ERR_INVALID_ARGUMENT, f"key {tuple(key.shape)} {key.dtype}, value {tuple(value.shape)} "
+                      f"{value.dtype}: contiguous, of one type")
+    _check_pools(k_cache, v_cache, k_scales, v_scales, k_cache.shape[0], n_kv, D, k_cache.shape[3])
+    _check_ints(slot_mapping, (T,), "slot_mapping")
+    if dtype_code(k_cache) != FP8_E4M3:
+        raise TLError(ERR_INVALID_ARGUMENT, f"pools of {k_cache.dtype}, not uint8")
+    _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
+    check(lib.tl_reshape_and_cache_fp8_scaled(
+        _ptr(key), _ptr(value), dtype_code(key), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+        _ptr(slot_mapping), T, n_kv, D, k_cache.shape[3], k_cache.shape[0], _stream(stream)))
 
 
 def _block_bytes(pool):
