@@ -10,6 +10,10 @@
 // tensors' own type takes the result rounded once; an FP8 pool takes
 //   scale = max|row| / 448,  code = e4m3(row / scale)
 // of each row (one token of one kv head; the key as rotated, in fp32).
+// Prompts go through the tiles of tl_append_tiles.hpp, steps (few tokens, as a
+// rule each in a block of its own) through axes_step_kernel; what neither
+// takes (odd strides, alignments and block sizes) through axes_rows_kernel.
+#include "tl_append_tiles.hpp"
 #include "tl_device.hpp"
 #include "tl_fp8.hpp"
 #include "tl_internal.hpp"
@@ -18,27 +22,11 @@ namespace tl {
 
 namespace {
 
-// An fp32 result as computed, before its conversion to a 2-byte type (which
-// the compiler would otherwise fuse with the last fma, rounding once).
-__device__ __forceinline__ float fp32_result(float r) {
-  asm volatile("" : "+v"(r));
-  return r;
-}
-
-// Whether token t is at a place of the tables on every axis.
-__device__ __forceinline__ bool placed(const AxesAppend& a, int64_t t) {
-  for (int x = 0; x < a.num_axes; ++x) {
-    const int pos = a.positions[x * (int64_t)a.num_tokens + t];
-    if (pos < 0 || pos >= a.max_positions) return false;
-  }
-  return true;
-}
-
 // Any size, stride and alignment: a wavefront per row (one head of one
 // token), lane l with pairs l and l + 64 (head_size at most 256); a row of
 // the value is taken as pairs too.
 template <Kind K, Kind POOL>
-__global__ __launch_bounds__(256) void axes_rows_kernel(AxesAppend a, int64_t row0) {
+__global__ __launch_bounds__(256) void axes_rows_kernel(TileAppend a, int style, int64_t row0) {
   const int lane = threadIdx.x % kWave, half = a.head_size / 2;
   const int per_token = a.num_heads + 2 * a.num_kv_heads;
   const int64_t row = row0 + (int64_t)blockIdx.x * (256 / kWave) + threadIdx.x / kWave;
@@ -63,7 +51,7 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(AxesAppend a, int64_t ro
   for (int j = 0; j < 2; ++j) {
     const int i = lane + kWave * j;
     if (i >= half) continue;
-    const int e0 = a.style == 0 ? 2 * i : i, e1 = a.style == 0 ? 2 * i + 1 : i + half;
+    const int e0 = style == 0 ? 2 * i : i, e1 = style == 0 ? 2 * i + 1 : i + half;
     const float x0 = load_scalar<K>(src, from + e0), x1 = load_scalar<K>(src, from + e1);
     x[j][0] = x0;
     x[j][1] = x1;
@@ -82,8 +70,8 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(AxesAppend a, int64_t ro
     for (int j = 0; j < 2; ++j) {
       const int i = lane + kWave * j;
       if (i >= half) continue;
-      store_scalar<K>(a.q_out, to + (a.style == 0 ? 2 * i : i), x[j][0]);
-      store_scalar<K>(a.q_out, to + (a.style == 0 ? 2 * i + 1 : i + half), x[j][1]);
+      store_scalar<K>(a.q_out, to + (style == 0 ? 2 * i : i), x[j][0]);
+      store_scalar<K>(a.q_out, to + (style == 0 ? 2 * i + 1 : i + half), x[j][1]);
     }
     return;
   }
@@ -99,8 +87,8 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(AxesAppend a, int64_t ro
   for (int j = 0; j < 2; ++j) {
     const int i = lane + kWave * j;
     if (i >= half) continue;
-    const int64_t d0 = to + (int64_t)(a.style == 0 ? 2 * i : i) * a.block_size;
-    const int64_t d1 = to + (int64_t)(a.style == 0 ? 2 * i + 1 : i + half) * a.block_size;
+    const int64_t d0 = to + (int64_t)(style == 0 ? 2 * i : i) * a.block_size;
+    const int64_t d1 = to + (int64_t)(style == 0 ? 2 * i + 1 : i + half) * a.block_size;
     if constexpr (POOL == Kind::FP8) {
       ((uint8_t*)pool)[d0] = f32_to_fp8(x[j][0] * scale.inv);
       ((uint8_t*)pool)[d1] = f32_to_fp8(x[j][1] * scale.inv);
@@ -111,14 +99,224 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(AxesAppend a, int64_t ro
   }
 }
 
-template <Kind K, Kind POOL>
-int launch_pool(const AxesAppend& a, hipStream_t stream) {
+// Steps: a wavefront per (token, kv head) with its key and its value, and
+// threads of 8 rotation pairs of a q head after them.  HBM has no byte masks:
+// storing a token's elements alone leaves partly written lines, each a
+// read-modify-write of memory later, so a lane rewrites the aligned SB bytes
+// of its channels' rows around the slot (the other slots with their own
+// bytes).  That needs them to be this token's: where another token of the
+// call writes into the same bytes, the elements are stored alone.
+// Lane l has the rotation pairs l and l + 64; its channels are theirs.
+template <int SB>
+struct RowBytes {
+  static constexpr int W = SB / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (SB == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const u32x4 v = load16(p + 16 * i);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* p) const {
+    if constexpr (SB == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i)
+        *reinterpret_cast<u32x4*>(p + 16 * i) = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    }
+  }
+  // element e of E bytes becomes v
+  template <int E>
+  __device__ __forceinline__ void put(int e, uint32_t v) {
+    const int at = e * E / 4, sh = 8 * (e * E % 4);
+    const uint32_t mask = (E == 4 ? 0xffffffffu : (1u << (8 * E % 32)) - 1u) << sh;
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = i == at ? (w[i] & ~mask) | (v << sh) : w[i];
+  }
+};
+
+constexpr int kStepMaxTokens = 256;      // a wavefront looks over the call's slots
+
+template <Kind K, Kind POOL, int ROPE, int SB>
+__global__ __launch_bounds__(kWave) void axes_step_kernel(TileAppend a) {
+  constexpr int E = KindInfo<POOL>::bytes, SLOTS = SB / E;
+  const int lane = threadIdx.x, half = a.head_size / 2;
+  if constexpr (ROPE != kNoRope) {
+    if ((int)blockIdx.x >= a.kv_wgs) {
+      const int units = half / 8;
+      const int64_t idx = ((int64_t)blockIdx.x - a.kv_wgs) * kWave + lane;
+      const int u = (int)(idx % units), h = (int)(idx / units % a.num_heads);
+      const int64_t t = idx / ((int64_t)units * a.num_heads);
+      if (t >= a.num_tokens) return;
+      float c[8], s[8], lo[8], hi[8];
+      load_unit<K, ROPE>(a.q, t * a.q_stride + h * a.head_size, u, half, lo, hi);
+      if (!placed(a, t)) return;                              // the token is left as it is
+      axes_turn(a, t, u, half, c, s);
+      rotate_unit<ROPE>(lo, hi, c, s);
+      store_unit<K, ROPE>(a.q_out, t * a.q_out_stride + h * a.head_size, u, half, lo, hi);
+      return;
+    }
+  }
+  const int t = blockIdx.x / a.num_kv_heads, h = blockIdx.x % a.num_kv_heads;
+  // everything that hangs on nothing else goes out first
+  const int32_t slot = a.slots[t];
+  int32_t others[kStepMaxTokens / kWave];
+#pragma unroll
+  for (int i = 0; i < kStepMaxTokens / kWave; ++i)
+    others[i] = kWave * i + lane < a.num_tokens ? a.slots[kWave * i + lane] : -1;
+  float k[2][2] = {}, v[2][2] = {};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane + kWave * j;
+    if (i >= half) break;
+    const int e0 = rope_channel<ROPE>(i, 0, half), e1 = rope_channel<ROPE>(i, 1, half);
+    const int64_t fk = t * a.key_stride + h * a.head_size, fv = t * a.value_stride + h * a.head_size;
+    k[j][0] = load_scalar<K>(a.key, fk + e0);
+    k[j][1] = load_scalar<K>(a.key, fk + e1);
+    v[j][0] = load_scalar<K>(a.value, fv + e0);
+    v[j][1] = load_scalar<K>(a.value, fv + e1);
+  }
+  if (ROPE != kNoRope && !placed(a, t)) return;
+  if (slot < 0 || slot / a.block_size >= a.num_blocks) return;
+  const int blk = slot / a.block_size, off = slot % a.block_size;
+  const int64_t head = (int64_t)blk * a.num_kv_heads + h;
+  char* kp = a.k_cache + (head * a.head_size * a.block_size + off / SLOTS * SLOTS) * E;
+  char* vp = a.v_cache + (head * a.head_size * a.block_size + off / SLOTS * SLOTS) * E;
+  const int64_t channel = (int64_t)a.block_size * E;
+  // whether the bytes around the slot are this token's alone
+  bool other = false;
+#pragma unroll
+  for (int i = 0; i < kStepMaxTokens / kWave; ++i)
+    other |= others[i] >= 0 && others[i] / SLOTS == slot / SLOTS && kWave * i + lane != t;
+  const bool alone = __builtin_amdgcn_ballot_w64(other) == 0;
+  RowBytes<SB> kr[2][2], vr[2][2];
+  if (alone) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (lane + kWave * j >= half) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int64_t c = rope_channel<ROPE>(lane + kWave * j, r, half) * channel;
+        kr[j][r].load(kp + c);
+        vr[j][r].load(vp + c);
+      }
+    }
+  }
+  uint32_t kt = 0, vt = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane + kWave * j;
+    if (i >= half) break;
+    if constexpr (ROPE != kNoRope) {
+      const int axis = a.axis_of[i / 16] >> (2 * (i % 16)) & 3;
+      const int64_t at = (int64_t)a.positions[axis * (int64_t)a.num_tokens + t] * half + i;
+      const float c = a.cos_table[at], s = a.sin_table[at], x0 = k[j][0], x1 = k[j][1];
+      k[j][0] = fp32_result(__builtin_fmaf(x0, c, -(x1 * s)));
+      k[j][1] = fp32_result(__builtin_fmaf(x0, s, x1 * c));
+    }
+    kt = max(kt, max(abs_bits(k[j][0]), abs_bits(k[j][1])));
+    vt = max(vt, max(abs_bits(v[j][0]), abs_bits(v[j][1])));
+  }
+  Fp8Scale ks = {}, vs = {};
+  if constexpr (POOL == Kind::FP8) {
+    ks = fp8_scale_of(lanes_umax<kWave>(kt));
+    vs = fp8_scale_of(lanes_umax<kWave>(vt));
+    if (lane == 0) {
+      a.k_scales[head * a.block_size + off] = ks.scale;
+      a.v_scales[head * a.block_size + off] = vs.scale;
+    }
+  }
+  auto bits = [&](float x, const Fp8Scale& sc) -> uint32_t {
+    if constexpr (POOL == Kind::FP8) return f32_to_fp8(x * sc.inv);
+    else return scalar_bits<POOL>(x);
+  };
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (lane + kWave * j >= half) break;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t c = rope_channel<ROPE>(lane + kWave * j, r, half) * channel;
+      const uint32_t kb = bits(k[j][r], ks), vb = bits(v[j][r], vs);
+      if (alone) {
+        kr[j][r].template put<E>(off % SLOTS, kb);
+        vr[j][r].template put<E>(off % SLOTS, vb);
+        kr[j][r].store(kp + c);
+        vr[j][r].store(vp + c);
+      } else if constexpr (E == 1) {
+        *(uint8_t*)(kp + c + off % SLOTS) = (uint8_t)kb;
+        *(uint8_t*)(vp + c + off % SLOTS) = (uint8_t)vb;
+      } else if constexpr (E == 2) {
+        *(uint16_t*)(kp + c + off % SLOTS * E) = (uint16_t)kb;
+        *(uint16_t*)(vp + c + off % SLOTS * E) = (uint16_t)vb;
+      } else {
+        *(uint32_t*)(kp + c + off % SLOTS * E) = kb;
+        *(uint32_t*)(vp + c + off % SLOTS * E) = vb;
+      }
+    }
+  }
+}
+
+template <Kind K, Kind POOL, int ROPE>
+int launch_style(const TileAppend& a, int style, hipStream_t stream) {
+  constexpr int E = KindInfo<POOL>::bytes, S = KindInfo<K>::bytes;
+  const auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  const auto whole = [](int64_t stride) { return stride * S % 16 == 0; };
+  const bool rows16 = ROPE == kNoRope || a.num_heads == 0 ||
+                      (al(a.q) && al(a.q_out) && whole(a.q_stride) && whole(a.q_out_stride));
+  const bool tables16 = ROPE == kNoRope || (al(a.cos_table) && al(a.sin_table));
+  const bool pools16 = al(a.k_cache) && al(a.v_cache);
+  if (a.num_tokens <= kStepMaxTokens && rows16 && tables16 && pools16) {
+    // the bytes of a channel's row around a slot: up to 64
+    const int row = a.block_size * E;
+    const int sb = row % 64 == 0 ? 64 : row == 32 || row == 16 || row == 8 ? row : 0;
+    TileAppend s = a;
+    s.kv_wgs = a.num_tokens * a.num_kv_heads;
+    const int64_t q = ROPE == kNoRope ? 0 : (int64_t)a.num_tokens * a.num_heads * (a.head_size / 16);
+    const int64_t wgs = (int64_t)a.num_tokens * a.num_kv_heads + (q + kWave - 1) / kWave;
+    if (sb && wgs < (1ll << 32) / kWave) {
+      const dim3 grid((unsigned)wgs);
+      auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kWave), 0, stream, s); };
+      if (sb == 64) go(axes_step_kernel<K, POOL, ROPE, 64>);
+      else if (sb == 32) go(axes_step_kernel<K, POOL, ROPE, 32>);
+      else if (sb == 16) go(axes_step_kernel<K, POOL, ROPE, 16>);
+      else go(axes_step_kernel<K, POOL, ROPE, 8>);
+      return hipGetLastError() == hipSuccess ? 0 : 5;
+    }
+  }
+  if (a.num_tokens > kStepMaxTokens && rows16 && whole(a.key_stride) && whole(a.value_stride) &&
+      tile_shape(a, S, E, ROPE != kNoRope))
+    return launch_tiles<K, POOL, ROPE, true>(a, stream);
   const int64_t rows = (int64_t)a.num_tokens * (a.num_heads + 2 * a.num_kv_heads), wgs = (rows + 3) / 4;
   constexpr int64_t kWgs = 1 << 23;                   // of a launch: fewer than 2^32 threads
   for (int64_t w = 0; w < wgs; w += kWgs)
     hipLaunchKernelGGL((axes_rows_kernel<K, POOL>), dim3((unsigned)(wgs - w < kWgs ? wgs - w : kWgs)), dim3(256), 0,
-                       stream, a, 4 * w);
+                       stream, a, style, 4 * w);
   return hipGetLastError() == hipSuccess ? 0 : 5;
+}
+
+template <Kind K, Kind POOL>
+int launch_pool(const AxesAppend& c, hipStream_t stream) {
+  TileAppend a = {};
+  a.q = c.q; a.q_out = c.q_out; a.key = c.key; a.value = c.value;
+  a.k_cache = (char*)c.k_cache; a.v_cache = (char*)c.v_cache;
+  a.k_scales = c.k_scales; a.v_scales = c.v_scales;
+  a.slots = c.slots; a.positions = c.positions; a.cos_table = c.cos_table; a.sin_table = c.sin_table;
+  a.num_tokens = c.num_tokens; a.num_heads = c.num_heads; a.num_kv_heads = c.num_kv_heads;
+  a.head_size = c.head_size; a.block_size = c.block_size; a.num_blocks = c.num_blocks;
+  a.max_positions = c.max_positions;
+  a.q_stride = c.q_stride; a.q_out_stride = c.q_out_stride;
+  a.key_stride = c.key_stride; a.value_stride = c.value_stride;
+  a.num_axes = c.num_axes;
+  for (int i = 0; i < 8; ++i) a.axis_of[i] = c.axis_of[i];
+  if (c.num_axes == 0) return launch_style<K, POOL, kNoRope>(a, 0, stream);
+  return c.style ? launch_style<K, POOL, 1>(a, 1, stream) : launch_style<K, POOL, 0>(a, 0, stream);
 }
 
 }  // namespace
