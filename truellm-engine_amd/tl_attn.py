@@ -259,23 +259,30 @@ def _torch():
     return torch
 
 
+_CODE_OF = {}             # torch dtype -> tl_dtype
+
+
 def dtype_code(t) -> int:
-    torch = _torch()
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.uint8: FP8_E4M3}
-    if t.dtype not in m:
+    if not _CODE_OF:
+        torch = _torch()
+        _CODE_OF.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.uint8: FP8_E4M3})
+    code = _CODE_OF.get(t.dtype)
+    if code is None:
         raise TLError(ERR_INVALID_ARGUMENT, f"unsupported tensor dtype {t.dtype}")
-    return m[t.dtype]
+    return code
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _on_gpu(*tensors):
     """Refuses tensors (None aside) that are not on the current device, whose streams and kernels would not reach
     them."""
+    first = tensors[0]
+    here = _torch().cuda.current_device() if first.is_cuda else -2
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.get_device() == _torch().cuda.current_device()):
+        if t is not None and t.get_device() != here:
             raise TLError(ERR_INVALID_ARGUMENT, f"a tensor on {t.device}, not on the current GPU")
 
 
@@ -378,20 +385,21 @@ def fused_add_rms_norm(out, residual, x, weight, eps, stream=None):
 
 
 def _norm_fp8_sizes(out, scales, x, weight, group_size, residual=None):
-    """(T, H) of an FP8 norm's tensors, whose sizes the library cannot see."""
-    T, H = x.shape
+    """(T, H, dtype) of an FP8 norm's tensors, whose sizes the library cannot see."""
+    shape, dtype = x.shape, x.dtype
+    T, H = shape
     want = (T, H // group_size) if group_size > 0 else (T,)
-    code = dtype_code(x)
-    if not (x.is_contiguous() and out.is_contiguous() and scales.is_contiguous() and out.shape == x.shape
-            and out.element_size() == 1 and tuple(scales.shape) == want and scales.element_size() == 4
-            and weight.numel() == H and weight.dtype == x.dtype and weight.is_contiguous()):
-        raise TLError(ERR_INVALID_ARGUMENT, f"x {tuple(x.shape)} {x.dtype}: out {tuple(out.shape)} {out.dtype}, "
-                      f"scales {tuple(scales.shape)} (fp32 {want}), weight {tuple(weight.shape)} {weight.dtype}")
-    if residual is not None and not (residual.shape == x.shape and residual.dtype == x.dtype
+    if not (out.shape == shape and out.element_size() == 1 and scales.shape == want and weight.shape == (H,)
+            and weight.dtype == dtype and dtype_code(scales) == F32 and x.is_contiguous() and out.is_contiguous()
+            and scales.is_contiguous() and weight.is_contiguous()):
+        raise TLError(ERR_INVALID_ARGUMENT, f"x {tuple(shape)} {dtype}: out {tuple(out.shape)} {out.dtype}, "
+                      f"scales {tuple(scales.shape)} {scales.dtype} (fp32 {want}), weight {tuple(weight.shape)} "
+                      f"{weight.dtype}, all contiguous")
+    if residual is not None and not (residual.shape == shape and residual.dtype == dtype
                                      and residual.is_contiguous()):
         raise TLError(ERR_INVALID_ARGUMENT, f"residual {tuple(residual.shape)} {residual.dtype}")
-    _on_gpu(out, scales, x, weight, residual)
-    return T, H, code
+    _on_gpu(x, out, scales, weight, residual)
+    return T, H, dtype_code(x)
 
 
 def rms_norm_fp8(out, scales, x, weight, eps, group_size=0, stream=None):
@@ -476,32 +484,32 @@ def make_rope_axes_desc(q, key, k_cache, axis_pairs, max_positions, *, style=ROP
     return d
 
 
-def _token_stride(t, heads, head_size, dtype, what):
+def _token_stride(t, T, heads, head_size, dtype, what):
     """Elements from a token of t [T, heads, head_size] to the next; its heads lie together."""
-    T = t.shape[0]
-    if (tuple(t.shape[1:]) != (heads, head_size) or dtype_code(t) != dtype or t.stride(2) != 1
-            or (heads > 1 and t.stride(1) != head_size) or (T > 1 and t.stride(0) < heads * head_size)):
-        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} strides {t.stride()}: "
-                      f"[T, {heads}, {head_size}] with the heads of a token together")
-    return t.stride(0) if T > 1 else 0
+    st = t.stride()
+    if (t.shape != (T, heads, head_size) or dtype_code(t) != dtype or st[2] != 1
+            or (heads > 1 and st[1] != head_size) or (T > 1 and st[0] < heads * head_size)):
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} strides {st}: "
+                      f"{(T, heads, head_size)} with the heads of a token together")
+    return st[0] if T > 1 else 0
 
 
-def _check_pools(k_cache, v_cache, k_scales, v_scales, num_blocks, heads, head_size, block_size):
+def _check_pools(k_cache, v_cache, k_scales, v_scales, kv_dtype, num_blocks, heads, head_size, block_size):
     """Pools [N, n_kv, D, bs] of one type, and their scales (None: none) fp32 [N, n_kv, bs]."""
     shape = (num_blocks, heads, head_size, block_size)
-    if not (tuple(k_cache.shape) == shape and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
-            and k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if not (k_cache.shape == shape and v_cache.shape == shape and dtype_code(k_cache) == kv_dtype
+            and v_cache.dtype == k_cache.dtype and k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise TLError(ERR_INVALID_ARGUMENT, f"pools {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} "
-                      f"{v_cache.dtype}: contiguous {shape} of one type")
+                      f"{v_cache.dtype}: contiguous {shape} of tl_dtype {kv_dtype}")
     for s in (k_scales, v_scales):
-        if s is not None and not (tuple(s.shape) == (num_blocks, heads, block_size) and dtype_code(s) == F32
+        if s is not None and not (s.shape == (num_blocks, heads, block_size) and dtype_code(s) == F32
                                   and s.is_contiguous()):
             raise TLError(ERR_INVALID_ARGUMENT, f"scales {tuple(s.shape)} {s.dtype}: contiguous fp32 "
                           f"{(num_blocks, heads, block_size)}")
 
 
 def _check_ints(t, shape, what):
-    if tuple(t.shape) != shape or t.dtype != _torch().int32 or not t.is_contiguous():
+    if t.shape != shape or t.dtype != _torch().int32 or not t.is_contiguous():
         raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype}: contiguous int32 {shape}")
 
 
@@ -510,28 +518,25 @@ def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_ca
     """RoPE with a position on each axis, positions int32 [axes, T], of q (into q_out, default in place) and key, then
     key/value into the pools; FP8 pools (uint8) take k_scales / v_scales fp32 [N, n_kv, bs], one scale per token and
     head.  q, q_out, key and value may be slices of a wider tensor (their token strides are read)."""
-    T, H, n_kv, D = key.shape[0], desc.num_heads, desc.num_kv_heads, desc.head_size
+    T, H, n_kv, D, dtype = key.shape[0], desc.num_heads, desc.num_kv_heads, desc.head_size, desc.dtype
     q_out = q if q_out is None else q_out
-    strides = [0, 0]
+    sq = so = 0
     if H:
-        strides = [_token_stride(q, H, D, desc.dtype, "q"), _token_stride(q_out, H, D, desc.dtype, "q_out")]
-        if q.shape[0] != T or q_out.shape[0] != T:
-            raise TLError(ERR_INVALID_ARGUMENT, f"q has {q.shape[0]}, q_out {q_out.shape[0]} tokens, key {T}")
-    strides += [_token_stride(key, n_kv, D, desc.dtype, "key"), _token_stride(value, n_kv, D, desc.dtype, "value")]
-    _check_pools(k_cache, v_cache, k_scales, v_scales, desc.num_blocks, n_kv, D, desc.block_size)
+        sq, so = _token_stride(q, T, H, D, dtype, "q"), _token_stride(q_out, T, H, D, dtype, "q_out")
+    sk, sv = _token_stride(key, T, n_kv, D, dtype, "key"), _token_stride(value, T, n_kv, D, dtype, "value")
+    _check_pools(k_cache, v_cache, k_scales, v_scales, desc.kv_dtype, desc.num_blocks, n_kv, D, desc.block_size)
     _check_ints(slot_mapping, (T,), "slot_mapping")
     _check_ints(positions, (desc.num_axes, T), "positions")
     table = (desc.max_positions, D // 2)
-    if value.shape[0] != T or dtype_code(k_cache) != desc.kv_dtype or any(
-            tuple(t.shape) != table or dtype_code(t) != F32 or not t.is_contiguous() for t in (cos_table, sin_table)):
-        raise TLError(ERR_INVALID_ARGUMENT, f"value has {value.shape[0]} tokens of {T}, pools {k_cache.dtype}, tables "
-                      f"{tuple(cos_table.shape)}, {tuple(sin_table.shape)} (fp32 {table})")
-    _on_gpu(q if H else None, q_out if H else None, key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping,
+    for t in (cos_table, sin_table):
+        if t.shape != table or dtype_code(t) != F32 or not t.is_contiguous():
+            raise TLError(ERR_INVALID_ARGUMENT, f"table {tuple(t.shape)} {t.dtype}: contiguous fp32 {table}")
+    _on_gpu(key, value, q if H else None, q_out if H else None, k_cache, v_cache, k_scales, v_scales, slot_mapping,
             positions, cos_table, sin_table)
     check(lib.tl_rope_axes_reshape_and_cache(
         ctypes.byref(desc), _ptr(q), _ptr(q_out), _ptr(key), _ptr(value), _ptr(k_cache), _ptr(v_cache),
         _ptr(k_scales), _ptr(v_scales), _ptr(slot_mapping), _ptr(positions), _ptr(cos_table), _ptr(sin_table), T,
-        *strides, _stream(stream)))
+        sq, so, sk, sv, _stream(stream)))
 
 
 def reshape_and_cache_fp8_scaled(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, stream=None):
@@ -541,10 +546,8 @@ def reshape_and_cache_fp8_scaled(key, value, k_cache, v_cache, k_scales, v_scale
     if not (key.is_contiguous() and value.is_contiguous() and value.shape == key.shape and value.dtype == key.dtype):
         raise TLError(ERR_INVALID_ARGUMENT, f"key {tuple(key.shape)} {key.dtype}, value {tuple(value.shape)} "
                       f"{value.dtype}: contiguous, of one type")
-    _check_pools(k_cache, v_cache, k_scales, v_scales, k_cache.shape[0], n_kv, D, k_cache.shape[3])
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, k_cache.shape[0], n_kv, D, k_cache.shape[3])
     _check_ints(slot_mapping, (T,), "slot_mapping")
-    if dtype_code(k_cache) != FP8_E4M3:
-        raise TLError(ERR_INVALID_ARGUMENT, f"pools of {k_cache.dtype}, not uint8")
     _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
     check(lib.tl_reshape_and_cache_fp8_scaled(
         _ptr(key), _ptr(value), dtype_code(key), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
