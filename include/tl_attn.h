@@ -110,6 +110,22 @@ int tl_paged_attention_decode(const tl_decode_desc* desc, void* out, const void*
                               int32_t max_context_len, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* No counterpart in the reference.  tl_paged_attention_decode over FP8 pools
+ * with a scale for each token and kv head (tl_reshape_and_cache_fp8_scaled,
+ * tl_rope_axes_reshape_and_cache): k_scales / v_scales fp32 [N, n_kv,
+ * block_size] beside the pools,
+ *   s_t = scale * k_scales_t (q . kcode_t),
+ *   out = sum_t softmax(s)_t v_scales_t vcode_t.
+ * desc->kv_dtype FP8_E4M3, head_size 128; k_scale / v_scale are ignored.  The
+ * plan and the workspace (tl_paged_attention_workspace_bytes) are those of
+ * the call without scales.  Scales past a sequence's length or in blocks that
+ * it does not name may hold anything.  A value of scale NaN makes its
+ * sequence's heads NaN, a key of scale NaN leaves them unspecified. */
+int tl_paged_attention_decode_scaled(const tl_decode_desc* desc, void* out, const void* q, const void* k_cache,
+                                     const void* v_cache, const float* k_scales, const float* v_scales,
+                                     const int32_t* block_tables, const int32_t* seq_lens, int32_t max_context_len,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* The engine's decode step in one call: reshape_and_cache of the step's
  * token then paged attention (cuda_engine.cpp:1100-1166), with the result
  * of tl_reshape_and_cache (tl_reshape_and_cache_fp8 for an FP8 pool, with

@@ -165,3 +165,60 @@ def test_append_bindings_refuse_wrong_tensors():
         a = {**good, **kw}
         with pytest.raises(tla.TLError):
             tla.reshape_and_cache_fp8_scaled(a["key"], a["value"], a["k"], a["v"], a["ks"], a["vs"], a["slots"])
+
+
+def _decode_desc(**kw):
+    d = tla.DecodeDesc()
+    d.num_seqs, d.num_heads, d.num_kv_heads, d.head_size, d.block_size = 4, 32, 8, 128, 16
+    d.max_blocks_per_seq, d.num_blocks, d.q_dtype, d.kv_dtype = 64, 512, tla.BF16, tla.FP8_E4M3
+    d.gqa_map, d.partition_tokens, d.scale = tla.GQA_GROUPED, 0, 0.088
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _decode(d, out=FAKE, q=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, bt=FAKE, sl=FAKE, ctx=1024, ws=None, ws_bytes=0):
+    return L.tl_paged_attention_decode_scaled(None if d is None else ctypes.byref(d), out, q, k, v, ks, vs, bt, sl, ctx, ws,
+                                              ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(kv_dtype=tla.BF16), tla.ERR_INVALID_ARGUMENT), (dict(kv_dtype=0, q_dtype=0), tla.ERR_INVALID_ARGUMENT),
+    (dict(q_dtype=tla.F32), tla.ERR_NOT_IMPLEMENTED), (dict(head_size=64), tla.ERR_NOT_IMPLEMENTED),
+    (dict(head_size=256), tla.ERR_NOT_IMPLEMENTED), (dict(block_size=12), tla.ERR_NOT_IMPLEMENTED),
+    (dict(block_size=512), tla.ERR_NOT_IMPLEMENTED), (dict(num_heads=30), tla.ERR_INVALID_ARGUMENT),
+    (dict(num_kv_heads=0), tla.ERR_INVALID_ARGUMENT), (dict(num_blocks=0), tla.ERR_INVALID_ARGUMENT),
+    (dict(gqa_map=2), tla.ERR_INVALID_ARGUMENT), (dict(partition_tokens=100), tla.ERR_INVALID_ARGUMENT),
+    (dict(num_seqs=-1), tla.ERR_INVALID_ARGUMENT)])
+def test_scaled_decode_refuses_descriptors(kw, code):
+    assert _decode(_decode_desc(**kw)) == code
+    assert tla.last_error()
+
+
+def test_scaled_decode_refuses_arguments():
+    d = _decode_desc()
+    assert _decode(None) == tla.ERR_INVALID_ARGUMENT
+    for name in ("out", "q", "k", "v", "ks", "vs", "bt", "sl"):
+        assert _decode(d, **{name: None}) == tla.ERR_INVALID_ARGUMENT, name
+    for name in ("k", "v", "ks", "vs"):
+        assert _decode(d, **{name: ctypes.c_void_p(0x1002)}) == tla.ERR_INVALID_ARGUMENT, name
+    assert _decode(d, ctx=-1) == tla.ERR_INVALID_ARGUMENT
+    assert _decode(_decode_desc(partition_tokens=256)) == tla.ERR_INVALID_ARGUMENT      # no workspace
+    assert _decode(_decode_desc(partition_tokens=256), ws=FAKE, ws_bytes=64) == tla.ERR_INVALID_ARGUMENT
+    assert _decode(_decode_desc(num_seqs=0), out=None, q=None, k=None, v=None, ks=None, vs=None, bt=None, sl=None) == tla.OK
+
+
+def test_scaled_decode_binding_refuses_wrong_tensors():
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    good = dict(q=torch.zeros(3, 8, 128, dtype=bf), out=torch.zeros(3, 8, 128, dtype=bf),
+                k=torch.zeros(6, 2, 128, 16, dtype=u8), v=torch.zeros(6, 2, 128, 16, dtype=u8), ks=torch.zeros(6, 2, 16),
+                vs=torch.zeros(6, 2, 16), bt=torch.zeros(3, 5, dtype=i32), sl=torch.zeros(3, dtype=i32))
+    desc = tla.make_decode_desc(good["q"], good["k"], good["bt"], 2, 0.1)
+    for kw in (dict(q=good["q"][:2]), dict(q=good["q"].half()), dict(out=good["out"].float()),
+               dict(out=good["out"].transpose(0, 1)), dict(k=good["k"][:5]), dict(v=good["v"].view(6, 2, 16, 128)),
+               dict(ks=good["ks"][:, :1]), dict(vs=good["vs"].half()), dict(bt=good["bt"].long()),
+               dict(bt=good["bt"][:, :4]), dict(sl=good["sl"][:2]), dict()):            # the last: not on a GPU
+        a = {**good, **kw}
+        with pytest.raises(tla.TLError):
+            tla.paged_attention_decode_scaled(desc, a["out"], a["q"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["sl"],
+                                              80)

@@ -98,6 +98,15 @@ int check_decode(const tl_decode_desc* d) {
   return TL_OK;
 }
 
+// What FP8 pools with a scale for each token and head need.
+int check_scales(const float* k_scales, const float* v_scales, int32_t head_size) {
+  if (head_size != 128) return fail(TL_ERR_NOT_IMPLEMENTED, "scaled FP8 pools: head_size=%d (built: 128)", head_size);
+  if (!k_scales || !v_scales) return fail(TL_ERR_INVALID_ARGUMENT, "FP8 pools need k_scales and v_scales");
+  if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3)
+    return fail(TL_ERR_INVALID_ARGUMENT, "k_scales / v_scales misaligned");
+  return TL_OK;
+}
+
 // Split-K plan: partition size and count for a batch whose longest sequence
 // is max_ctx.  Aim for >= 512 workgroups (two per CU on 256 CUs, which is
 // what the single-pass kernels' occupancy admits); a batch that already
@@ -286,7 +295,8 @@ size_t tl_paged_attention_workspace_bytes(const tl_decode_desc* desc, int32_t ma
 static int decode_impl(const tl_decode_desc* desc, void* out, const void* q, const void* k_cache,
                        const void* v_cache, const int32_t* block_tables, const int32_t* seq_lens,
                        int32_t max_context_len, void* workspace, size_t workspace_bytes, void* stream,
-                       const void* key, const void* value, const int32_t* slots) {
+                       const void* key, const void* value, const int32_t* slots, const float* k_scales = nullptr,
+                       const float* v_scales = nullptr) {
   int rc = check_decode(desc);
   if (rc) return rc;
   if (max_context_len < 0) return fail(TL_ERR_INVALID_ARGUMENT, "max_context_len < 0");
@@ -301,6 +311,8 @@ static int decode_impl(const tl_decode_desc* desc, void* out, const void* q, con
   int P, PT;
   plan_partitions(desc, max_context_len, &P, &PT);
   tl::DecodeLaunch a = make_launch(desc, out, q, k_cache, v_cache, block_tables, seq_lens, stream);
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
   if (P > 1) {
     const size_t need = ws_bytes(desc, P);
     if (!workspace || workspace_bytes < need)
@@ -334,6 +346,23 @@ int tl_paged_attention_decode(const tl_decode_desc* desc, void* out, const void*
                               void* stream) {
   return decode_impl(desc, out, q, k_cache, v_cache, block_tables, seq_lens, max_context_len, workspace,
                      workspace_bytes, stream, nullptr, nullptr, nullptr);
+}
+
+int tl_paged_attention_decode_scaled(const tl_decode_desc* desc, void* out, const void* q, const void* k_cache,
+                                     const void* v_cache, const float* k_scales, const float* v_scales,
+                                     const int32_t* block_tables, const int32_t* seq_lens, int32_t max_context_len,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (!desc) return fail(TL_ERR_INVALID_ARGUMENT, "desc is NULL");
+  if (desc->kv_dtype != TL_DTYPE_FP8_E4M3)
+    return fail(TL_ERR_INVALID_ARGUMENT, "kv_dtype=%d: scales of each token go with FP8_E4M3", desc->kv_dtype);
+  if (desc->num_seqs > 0) {
+    const int rc = check_scales(k_scales, v_scales, desc->head_size);
+    if (rc) return rc;
+  }
+  tl_decode_desc d = *desc;
+  d.k_scale = d.v_scale = 1.f;
+  return decode_impl(&d, out, q, k_cache, v_cache, block_tables, seq_lens, max_context_len, workspace,
+                     workspace_bytes, stream, nullptr, nullptr, nullptr, k_scales, v_scales);
 }
 
 int tl_paged_attention_decode_step(const tl_decode_desc* desc, void* out, const void* q, const void* key,
@@ -501,15 +530,6 @@ int tl_rope_reshape_and_cache(const void* q, void* q_out, const void* key, const
   const int rc = tl::launch_rope_cache(a, (hipStream_t)stream);
   if (rc) return fail(TL_ERR_BACKEND, "rope_reshape_and_cache launch failed");
   return ok();
-}
-
-// What FP8 pools with a scale for each token and head need.
-static int check_scales(const float* k_scales, const float* v_scales, int32_t head_size) {
-  if (head_size != 128) return fail(TL_ERR_NOT_IMPLEMENTED, "scaled FP8 pools: head_size=%d (built: 128)", head_size);
-  if (!k_scales || !v_scales) return fail(TL_ERR_INVALID_ARGUMENT, "FP8 pools need k_scales and v_scales");
-  if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3)
-    return fail(TL_ERR_INVALID_ARGUMENT, "k_scales / v_scales misaligned");
-  return TL_OK;
 }
 
 // Slots are int32: a pool past 2^31 of them has blocks that none can name.

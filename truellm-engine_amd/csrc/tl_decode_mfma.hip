@@ -11,7 +11,8 @@
 //     read, where the dot-product wavefront reads the KV once per 4 heads.
 // The dequant scales of FP8 fold into the score scale (k_scale) and the
 // output (v_scale), as the reference's dequantise-then-multiply does (the
-// scaled K/V are k_scale * code and v_scale * code).  Workgroups and the
+// scaled K/V are k_scale * code and v_scale * code); scales of each token
+// enter the scores and the weights (FP8S).  Workgroups and the
 // split-K / log-sum-exp protocol are those of the 2-byte decode (NW
 // wavefronts stride over a partition's iterations and merge in LDS).
 #include <algorithm>
@@ -58,13 +59,13 @@ __device__ __forceinline__ bool item_of(const Params& p, bool final, bool late_e
 // (item_of's late_exit), for grids that fit the GPU in one round, where the
 // launch is a chain of round trips (length, table, K/V, partials) and the
 // few loads of an exiting workgroup cost less than a round trip.
-template <Kind QK, Kind PO, int NW, bool FINAL, int BS, bool LATE = false>
+template <Kind KV, Kind QK, Kind PO, int NW, bool FINAL, int BS, bool LATE = false>
 __global__ __launch_bounds__(NW * kWave) void fp8_decode_kernel(Params p) {
   __shared__ __attribute__((aligned(16))) float s_acc[NW * mw::kHeads * mw::kHead];
   __shared__ float s_m[NW * mw::kHeads], s_l[NW * mw::kHeads];
   Item w;
   if (!item_of(p, FINAL, LATE, w)) return;
-  mw::decode_workgroup<Kind::FP8, QK, PO, NW, FINAL, BS, LATE>(p, w.seq, w.kvh, w.hs, w.part, w.t0, w.t1, s_acc,
+  mw::decode_workgroup<KV, QK, PO, NW, FINAL, BS, LATE>(p, w.seq, w.kvh, w.hs, w.part, w.t0, w.t1, s_acc,
                                                                s_m, s_l, w.len);
 }
 
@@ -122,8 +123,8 @@ template <Kind KV, Kind QK, int NW, bool FINAL, int BS, Kind PO_SPLIT = Kind::F3
           int ITERS = 0>
 void launch_kernel(const Params& p, unsigned grid, hipStream_t stream) {
   constexpr Kind PO = FINAL ? QK : PO_SPLIT;
-  if constexpr (KV == Kind::FP8)
-    hipLaunchKernelGGL((fp8_decode_kernel<QK, PO, NW, FINAL, BS, LATE>), dim3(grid), dim3(NW * kWave), 0, stream,
+  if constexpr (is_fp8<KV>())
+    hipLaunchKernelGGL((fp8_decode_kernel<KV, QK, PO, NW, FINAL, BS, LATE>), dim3(grid), dim3(NW * kWave), 0, stream,
                        p);
   else
     hipLaunchKernelGGL((mfma2_decode_kernel<KV, PO, NW, FINAL, BS, LATE, ITERS>), dim3(grid), dim3(NW * kWave), 0,
@@ -135,9 +136,9 @@ void launch_kernel(const Params& p, unsigned grid, hipStream_t stream) {
 template <Kind KV, Kind QK, int NW, int BS, Kind PO_SPLIT>
 void launch_late(const Params& p, unsigned grid, hipStream_t stream) {
   const int step = NW * mw::tokens_per_iteration<KV>();
-  if (KV != Kind::FP8 && p.partition_tokens <= step)
+  if (!is_fp8<KV>() && p.partition_tokens <= step)
     launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 1>(p, grid, stream);
-  else if (KV != Kind::FP8 && p.partition_tokens <= 2 * step)
+  else if (!is_fp8<KV>() && p.partition_tokens <= 2 * step)
     launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 2>(p, grid, stream);
   else
     launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 0>(p, grid, stream);
@@ -160,6 +161,7 @@ int launch_typed(const DecodeLaunch& a) {
   const bool fp8 = KV == Kind::FP8;
   p.qk_scale = a.scale * (fp8 ? a.k_scale : 1.f) * kLog2e;
   p.v_scale = fp8 ? a.v_scale : 1.f;
+  p.k_scales = a.k_scales; p.v_scales = a.v_scales;
   const int P = a.num_partitions;
   const unsigned items = (unsigned)(a.num_seqs * a.num_kv_heads * p.head_slices);
   if (P == 1) {
@@ -233,6 +235,9 @@ int launch_decode_mfma(const DecodeLaunch& a) {
   if (!decode_uses_mfma(a.kv_dtype, a.num_heads, a.num_kv_heads, a.head_size, a.block_size)) return 3;
   const int tpi = kv == Kind::FP8 ? mw::tokens_per_iteration<Kind::FP8>() : mw::tokens_per_iteration<Kind::F16>();
   if (a.num_partitions > 1 && a.partition_tokens % tpi) return 3;
+  if (kv == Kind::FP8 && a.k_scales)
+    return qk == Kind::F16 ? launch_bs<Kind::FP8S, Kind::F16>(a)
+                           : qk == Kind::BF16 ? launch_bs<Kind::FP8S, Kind::BF16>(a) : 3;
   if (kv == Kind::FP8 && qk == Kind::F16) return launch_bs<Kind::FP8, Kind::F16>(a);
   if (kv == Kind::FP8 && qk == Kind::BF16) return launch_bs<Kind::FP8, Kind::BF16>(a);
   if (kv == Kind::F16 && qk == Kind::F16) return launch_bs<Kind::F16, Kind::F16>(a);

@@ -49,6 +49,9 @@ struct Params {
   float qk_scale;  // softmax scale * k dequant scale * log2(e)
   float v_scale;
   int block_size = 0;   // pool block size, read by kernels built for any block size
+  // FP8S pools: the scales [N, n_kv, block size]
+  const float* k_scales = nullptr;
+  const float* v_scales = nullptr;
 };
 
 // The work item of a decode workgroup: returns the index of its (sequence,

@@ -14,13 +14,17 @@ constexpr int kWave = 64;
 // Storage kinds of the KV pool.  F16/BF16/F32 follow truellm::DataType
 // (include/truellm/types.h:47-60); FP8 is OCP E4M3 ("E4M3FN", max 448), the
 // format gfx950's v_cvt_*_fp8 instructions implement.
-enum class Kind : int { F32 = 0, F16 = 1, BF16 = 2, FP8 = 32 };
+// FP8S: FP8 codes under a scale for each token and kv head, in arrays beside
+// the pools (FP8: one scale for each pool).
+enum class Kind : int { F32 = 0, F16 = 1, BF16 = 2, FP8 = 32, FP8S = 33 };
+template <Kind K> constexpr bool is_fp8() { return K == Kind::FP8 || K == Kind::FP8S; }
 
 template <Kind K> struct KindInfo;
 template <> struct KindInfo<Kind::F32>  { static constexpr int bytes = 4; };
 template <> struct KindInfo<Kind::F16>  { static constexpr int bytes = 2; };
 template <> struct KindInfo<Kind::BF16> { static constexpr int bytes = 2; };
 template <> struct KindInfo<Kind::FP8>  { static constexpr int bytes = 1; };
+template <> struct KindInfo<Kind::FP8S> { static constexpr int bytes = 1; };
 
 typedef float  f32x2 __attribute__((ext_vector_type(2)));
 typedef float  f32x4 __attribute__((ext_vector_type(4)));
@@ -216,6 +220,7 @@ constexpr int kDppXor1 = 0xB1;         // quad_perm [1,0,3,2]
 constexpr int kDppXor2 = 0x4E;         // quad_perm [2,3,0,1]
 constexpr int kDppHalfMirror = 0x141;  // lane i <- 7 - i within each 8 lanes
 constexpr int kDppMirror = 0x140;      // lane i <- 15 - i within each row
+constexpr int kDppLane0 = 0x150;       // + n: every lane of a row <- its lane n
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));

@@ -28,6 +28,8 @@ struct DecodeLaunch {
   int partition_tokens;         // multiple of kDecodeChunk when P > 1
   int q_dtype, kv_dtype, gqa_map;
   float scale, k_scale, v_scale;
+  const float* k_scales;        // FP8 with a scale for each token and kv head [N, n_kv, BS], else null
+  const float* v_scales;
   int part_o_dtype;             // split-K partial outputs: F32 (0), or F16 (f16 q and KV, head 128)
   hipStream_t stream;
 };

@@ -40,7 +40,7 @@ constexpr int kHead = 128;
 constexpr int kHeads = 16;          // q heads per wavefront: the MFMA columns
 constexpr float kLazyRescale = 8.f; // rescale once the max grows by more than 2^8
 
-template <Kind KV> constexpr int tokens_per_iteration() { return KV == Kind::FP8 ? 64 : 32; }
+template <Kind KV> constexpr int tokens_per_iteration() { return is_fp8<KV>() ? 64 : 32; }
 
 // Two E4M3 codes (bytes 0,1 or 2,3 of w) to two f16, exactly.
 template <bool HI>
@@ -182,15 +182,17 @@ __device__ __forceinline__ u32x4 keep_halves(const u32x4& v, int n) {
 
 // The running softmax state of a wavefront and its hand-over to LDS
 // (s_acc_w [16][128] unnormalised, times v_scale; s_m_w [16] in log2 units;
-// s_l_w [16]).
+// s_l_w [16]).  o is in units of `unit`, a power of two (1 without scales of
+// each token).
 struct State {
   f4 o[8];
-  float m_run, l_lane;
+  float m_run, l_lane, unit;
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = f4{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
     l_lane = 0.f;
+    unit = 1.f;
   }
   // Raises the running max to the wavefront's new max mx when it grew by
   // more than 2^8 for some head.
@@ -204,12 +206,25 @@ struct State {
       m_run = m_new;
     }
   }
+  // Scales of values in a unit near the largest of them (v: this lane's token
+  // of the iteration): returns 1 / unit.
+  __device__ __forceinline__ float raise_unit(float v) {
+    const float top = max_kg(row_max(v));
+    if (top > 64.f * unit) {                           // the same in every lane; also where unit is 0
+      const float u = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, top) & 0x7f800000u);
+      const float f = unit / u;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
+      unit = u;
+    }
+    return unit > 0.f ? 1.f / unit : 0.f;
+  }
   __device__ __forceinline__ void store(float v_scale, int m, int kg, float* s_acc_w, float* s_m_w,
                                         float* s_l_w) const {
     const float l_tot = sum_kg(l_lane);
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
-      *reinterpret_cast<f4*>(&s_acc_w[m * kHead + 16 * dt + 4 * kg]) = o[dt] * v_scale;
+      *reinterpret_cast<f4*>(&s_acc_w[m * kHead + 16 * dt + 4 * kg]) = o[dt] * (v_scale * unit);
     if (kg == 0) {
       s_m_w[m] = m_run;
       s_l_w[m] = l_tot;
@@ -225,6 +240,22 @@ struct NoFlush {
   int part_tokens = 1;
   __device__ void operator()(const State&, int) const {}
 };
+
+// s[i][r] times x of lane 4 r + i of the row (the token whose score it is).
+template <int N>
+__device__ __forceinline__ float row_lane(float x) { return dpp<kDppLane0 + N>(x); }
+__device__ __forceinline__ void scale_scores(f4 (&s)[4], float x) {
+  s[0][0] *= row_lane<0>(x);  s[1][0] *= row_lane<1>(x);  s[2][0] *= row_lane<2>(x);  s[3][0] *= row_lane<3>(x);
+  s[0][1] *= row_lane<4>(x);  s[1][1] *= row_lane<5>(x);  s[2][1] *= row_lane<6>(x);  s[3][1] *= row_lane<7>(x);
+  s[0][2] *= row_lane<8>(x);  s[1][2] *= row_lane<9>(x);  s[2][2] *= row_lane<10>(x); s[3][2] *= row_lane<11>(x);
+  s[0][3] *= row_lane<12>(x); s[1][3] *= row_lane<13>(x); s[2][3] *= row_lane<14>(x); s[3][3] *= row_lane<15>(x);
+}
+__device__ __forceinline__ void scale_weights(float (&w)[4][4], float x) {
+  w[0][0] *= row_lane<0>(x);  w[1][0] *= row_lane<1>(x);  w[2][0] *= row_lane<2>(x);  w[3][0] *= row_lane<3>(x);
+  w[0][1] *= row_lane<4>(x);  w[1][1] *= row_lane<5>(x);  w[2][1] *= row_lane<6>(x);  w[3][1] *= row_lane<7>(x);
+  w[0][2] *= row_lane<8>(x);  w[1][2] *= row_lane<9>(x);  w[2][2] *= row_lane<10>(x); w[3][2] *= row_lane<11>(x);
+  w[0][3] *= row_lane<12>(x); w[1][3] *= row_lane<13>(x); w[2][3] *= row_lane<14>(x); w[3][3] *= row_lane<15>(x);
+}
 
 // ---- FP8 E4M3 KV, f16 / bf16 q: 64 tokens per iteration ----
 //
@@ -245,13 +276,23 @@ struct NoFlush {
 // |q| in [2^14, 2^15)); the factor returns in the score scale.  The
 // dequant scales fold into the score scale (k_scale) and the output
 // (v_scale).
-template <Kind QK, int BS, class Flush = NoFlush>
+//
+// FP8S (a scale for each token): lane l loads the key's and the value's scale
+// of iteration token l, one dword each, an iteration ahead.  The 16 lanes of
+// a row (kg) hold the scales of the 16 tokens whose scores they hold, so the
+// scale of token 4 r + i is a row broadcast (DPP, an operand of the multiply).
+// The score takes ks; the weight takes vs before it is rounded to f16, in
+// units of a power of two near the largest vs so far (State::unit, raised
+// when a vs passes 2^6 of it: weights stay below 2^14), so that values of any
+// size keep f16's precision.
+template <Kind KV, Kind QK, int BS, class Flush = NoFlush>
 __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int hs, int first_it, int t1,
                                           int step, const Flush& flush = Flush(), int len = 0x7fffffff) {
   static_assert(BS >= 8 && (BS & (BS - 1)) == 0, "block size: a power of two >= 8");
   t1 = min(t1, len);
   constexpr int TPI = 64, RB = BS;           // tokens per iteration; bytes per head-dim row of a block
   constexpr bool kSplitRun = BS == 8;        // a lane's 16-token V run spans two blocks
+  constexpr bool kScaled = KV == Kind::FP8S;
   constexpr int kBlockBytes = kHead * RB;
   constexpr int NB = blocks_per_iteration<BS, TPI>();
   const int lane = threadIdx.x % kWave;
@@ -351,6 +392,14 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
   auto v_at = [&](const Blocks<NB>& b, int ib, int which) {
     return vbase0 + ib + (int64_t)max(pick(b, which), 0) * pool_stride;
   };
+  // the scale of iteration token `lane`, in the iteration of entries b (a
+  // missing block reads block 0, as the loads above)
+  const int sb = NB > 1 ? lane / BS : 0, st_off = NB > 1 ? lane % BS : lane;
+  auto scale_at = [&](const float* scales, const Blocks<NB>& b, int ib) {
+    return scales[((int64_t)max(pick(b, sb), 0) * p.num_kv_heads + kvh) * BS + st_off + ib];
+  };
+  float ks = 0.f, vs = 0.f;
+  if constexpr (kScaled) st.unit = 0.f;               // none seen
 
   int it = first_it;
   Blocks<NB> cur = table_blocks<NB, BS>(p, table, it, t1);
@@ -362,6 +411,10 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
     // the loads in flight from its first iteration on
     const int ib = in_block_bytes<BS, TPI, 1>(it);
     load_k(kw, kbase0 + ib + (int64_t)max(pick(cur, kb), 0) * pool_stride);
+    if constexpr (kScaled) {
+      ks = scale_at(p.k_scales, cur, ib);
+      vs = scale_at(p.v_scales, cur, ib);
+    }
     __builtin_amdgcn_sched_barrier(0);
     load_v(vr, v_at(cur, ib, vb), v_at(cur, ib, vb2));
   }
@@ -372,6 +425,7 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       if (it != first_it && it % flush.part_tokens == 0) {   // a partition ends: its partials out, state afresh
         flush(st, it / flush.part_tokens - 1);
         st.init();
+        if constexpr (kScaled) st.unit = 0.f;
       }
     }
     const Blocks<NB> nn = table_blocks<NB, BS>(p, table, it + 2 * step, t1);
@@ -424,13 +478,15 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       n_ok = ph_v < 0 ? 0 : min(max(t1 - (it + 16 * kg), 0), 16);
     }
     auto tok_ok = [&](int t) { return kSplitRun ? ((keep >> t) & 1u) != 0 : t < n_ok; };
+    // (bf16: qk_scale is the head's, not the token's, and stays with the lane)
+    if constexpr (kScaled) scale_scores(s, QK == Kind::BF16 ? ks : ks * qk_scale);
     float sc[4][4];
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[i][r] = tok_ok(4 * r + i) ? s[i][r] * qk_scale : -INFINITY;
+        sc[i][r] = tok_ok(4 * r + i) ? (kScaled && QK != Kind::BF16 ? s[i][r] : s[i][r] * qk_scale) : -INFINITY;
         mx = fmaxf(mx, sc[i][r]);
       }
     st.update_max(mx);
@@ -442,6 +498,15 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
         pw[i][r] = tok_ok(4 * r + i) ? __builtin_amdgcn_exp2f(sc[i][r] - st.m_run) : 0.f;
         st.l_lane += pw[i][r];
       }
+    if constexpr (kScaled) {
+      // the lane's own token: past the end or in a hole its scale may be anything
+      const float v_own = pick(cur, sb) >= 0 && it + lane < t1 ? vs : 0.f;
+      const float inv = st.raise_unit(v_own);
+      scale_weights(pw, v_own * inv);
+      // the next iteration's, after this one's last use of the registers
+      ks = scale_at(p.k_scales, nxt, ib_next);
+      vs = scale_at(p.v_scales, nxt, ib_next);
+    }
     // P^T operands: MFMA h takes tokens 8 h .. 8 h + 7 = (r = 2 h, 2 h + 1) x (i = 0 .. 3)
     u4v pb[2];
 #pragma unroll
@@ -703,8 +768,8 @@ __device__ __forceinline__ State mfma2_wave(const Params& p, int seq, int kvh, i
 template <Kind KV, Kind QK, int BS, class Flush = NoFlush, int ITERS = 0>
 __device__ __forceinline__ State run_wave(const Params& p, int seq, int kvh, int hs, int first_it, int t1,
                                           int step, const Flush& flush = Flush(), int len = 0x7fffffff) {
-  if constexpr (KV == Kind::FP8)
-    return fp8_wave<QK, BS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
+  if constexpr (is_fp8<KV>())
+    return fp8_wave<KV, QK, BS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
   else
     return mfma2_wave<KV, BS, Flush, ITERS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
 }
@@ -720,7 +785,7 @@ struct Partial {
 };
 __device__ __forceinline__ Partial finish_partial(const State& st, float v_scale) {
   const float l_tot = sum_kg(st.l_lane);
-  const float f = l_tot > 0.f ? v_scale / l_tot : 0.f;
+  const float f = l_tot > 0.f ? v_scale * st.unit / l_tot : 0.f;
   Partial r;
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) r.o[dt] = st.o[dt] * f;

@@ -136,6 +136,8 @@ _SIG = {
     "tl_last_error_string": (ctypes.c_char_p, []),
     "tl_paged_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecodeDesc), _I]),
     "tl_paged_attention_decode": (ctypes.c_int, [ctypes.POINTER(DecodeDesc), _P, _P, _P, _P, _P, _P, _I, _P, ctypes.c_size_t, _P]),
+    "tl_paged_attention_decode_scaled": (ctypes.c_int, [ctypes.POINTER(DecodeDesc)] + [_P] * 8
+                                         + [_I, _P, ctypes.c_size_t, _P]),
     "tl_paged_attention_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(DecodeDesc), _P, _P, _P, _P, _P, _P, _I, _P]),
     "tl_paged_attention_v1": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
     "tl_paged_attention_v2": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P]),
@@ -623,6 +625,25 @@ def paged_attention_decode(desc: DecodeDesc, out, q, k_cache, v_cache, block_tab
     check(lib.tl_paged_attention_decode(
         ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
         _ptr(seq_lens), max_context_len, _ptr(workspace), ws_bytes, _stream(stream)))
+
+
+def paged_attention_decode_scaled(desc: DecodeDesc, out, q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
+                                  max_context_len, workspace=None, stream=None):
+    """paged_attention_decode over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
+    S = desc.num_seqs
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, desc.num_kv_heads, desc.head_size,
+                 desc.block_size)
+    _check_ints(block_tables, (S, desc.max_blocks_per_seq), "block_tables")
+    _check_ints(seq_lens, (S,), "seq_lens")
+    for t in (q, out):
+        if t.shape != (S, desc.num_heads, desc.head_size) or dtype_code(t) != desc.q_dtype or not t.is_contiguous():
+            raise TLError(ERR_INVALID_ARGUMENT, f"q / out {tuple(t.shape)} {t.dtype}: contiguous "
+                          f"{(S, desc.num_heads, desc.head_size)} of the descriptor's type")
+    _on_gpu(q, out, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, workspace)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(lib.tl_paged_attention_decode_scaled(
+        ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+        _ptr(block_tables), _ptr(seq_lens), max_context_len, _ptr(workspace), ws_bytes, _stream(stream)))
 
 
 NOALLOC_SCRATCH_BYTES = 32 << 20
