@@ -507,14 +507,24 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       ks = scale_at(p.k_scales, nxt, ib_next);
       vs = scale_at(p.v_scales, nxt, ib_next);
     }
-    // P^T operands: MFMA h takes tokens 8 h .. 8 h + 7 = (r = 2 h, 2 h + 1) x (i = 0 .. 3)
-    u4v pb[2];
+    // P^T operands: MFMA h takes tokens 8 h .. 8 h + 7 = (r = 2 h, 2 h + 1) x (i = 0 .. 3).
+    // Where out is f16 (kLow) the rest that rounding a weight to f16 leaves
+    // goes in a second f16: alone the weights' rounding would add as much
+    // again as the output's own (one sequence of 4096: 3.5e-4 off 64 bits
+    // against 2.0e-4), and the products are not what bounds this loop.
+    constexpr bool kLow = kScaled && QK == Kind::F16;
+    u4v pb[2], pl[kLow ? 2 : 1];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      h8 v;
+      h8 v, low;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (_Float16)pw[e & 3][2 * h + (e >> 2)];
+      for (int e = 0; e < 8; ++e) {
+        const float w = pw[e & 3][2 * h + (e >> 2)];
+        v[e] = (_Float16)w;
+        if constexpr (kLow) low[e] = (_Float16)(w - (float)v[e]);
+      }
       pb[h] = __builtin_bit_cast(u4v, v);
+      if constexpr (kLow) pl[h] = __builtin_bit_cast(u4v, low);
     }
 
     // ---- p.v: tokens past t1 and holes may hold any byte (NaN codes too) ----
@@ -530,10 +540,14 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
       const u32x4 v = vr[dt];
-      st.o[dt] = mma<Kind::F16>(f8x2<false>(v.x), f8x2<true>(v.x), f8x2<false>(v.y), f8x2<true>(v.y), pb[0],
-                                st.o[dt]);
-      st.o[dt] = mma<Kind::F16>(f8x2<false>(v.z), f8x2<true>(v.z), f8x2<false>(v.w), f8x2<true>(v.w), pb[1],
-                                st.o[dt]);
+      const uint32_t a[8] = {f8x2<false>(v.x), f8x2<true>(v.x), f8x2<false>(v.y), f8x2<true>(v.y),
+                             f8x2<false>(v.z), f8x2<true>(v.z), f8x2<false>(v.w), f8x2<true>(v.w)};
+      st.o[dt] = mma<Kind::F16>(a[0], a[1], a[2], a[3], pb[0], st.o[dt]);
+      st.o[dt] = mma<Kind::F16>(a[4], a[5], a[6], a[7], pb[1], st.o[dt]);
+      if constexpr (kLow) {
+        st.o[dt] = mma<Kind::F16>(a[0], a[1], a[2], a[3], pl[0], st.o[dt]);
+        st.o[dt] = mma<Kind::F16>(a[4], a[5], a[6], a[7], pl[1], st.o[dt]);
+      }
     }
     load_v(vr, v_at(nxt, ib_next, vb), v_at(nxt, ib_next, vb2));
     cur = nxt;
