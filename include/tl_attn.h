@@ -733,6 +733,15 @@ int tl_chunked_prefill(const tl_prefill_desc* desc, void* out, const void* q,
                        const int32_t* block_tables, const int32_t* seq_lens,
                        int32_t total_q, int32_t max_q_len, void* stream);
 
+/* tl_chunked_prefill over FP8 pools with a scale for each token and kv head
+ * (as tl_paged_attention_decode_scaled reads them; kv_dtype FP8_E4M3, k_scale
+ * / v_scale ignored).  A value or key of scale NaN makes outputs of its
+ * sequence's chunk NaN or unspecified in that head, of earlier rows too. */
+int tl_chunked_prefill_scaled(const tl_prefill_desc* desc, void* out, const void* q, const int32_t* cu_q_lens,
+                              const void* k_cache, const void* v_cache, const float* k_scales,
+                              const float* v_scales, const int32_t* block_tables, const int32_t* seq_lens,
+                              int32_t total_q, int32_t max_q_len, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

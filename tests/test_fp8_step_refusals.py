@@ -222,3 +222,56 @@ def test_scaled_decode_binding_refuses_wrong_tensors():
         with pytest.raises(tla.TLError):
             tla.paged_attention_decode_scaled(desc, a["out"], a["q"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["sl"],
                                               80)
+
+
+def _prefill_desc(**kw):
+    d = tla.PrefillDesc()
+    d.num_seqs, d.num_heads, d.num_kv_heads, d.head_size, d.block_size = 4, 32, 8, 128, 16
+    d.max_blocks_per_seq, d.num_blocks, d.dtype, d.kv_dtype = 64, 512, tla.BF16, tla.FP8_E4M3
+    d.gqa_map, d.scale = tla.GQA_GROUPED, 0.088
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _prefill(d, out=FAKE, q=FAKE, cu=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, bt=FAKE, sl=FAKE, total=64, most=32):
+    return L.tl_chunked_prefill_scaled(None if d is None else ctypes.byref(d), out, q, cu, k, v, ks, vs, bt, sl, total, most,
+                                       None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(kv_dtype=tla.BF16), tla.ERR_INVALID_ARGUMENT), (dict(kv_dtype=0), tla.ERR_INVALID_ARGUMENT),
+    (dict(dtype=tla.F32), tla.ERR_NOT_IMPLEMENTED), (dict(head_size=64), tla.ERR_NOT_IMPLEMENTED),
+    (dict(block_size=4), tla.ERR_NOT_IMPLEMENTED), (dict(block_size=24), tla.ERR_NOT_IMPLEMENTED),
+    (dict(num_heads=30), tla.ERR_INVALID_ARGUMENT), (dict(num_blocks=0), tla.ERR_INVALID_ARGUMENT),
+    (dict(num_prefill_seqs=5), tla.ERR_INVALID_ARGUMENT), (dict(scale=0.0), tla.ERR_INVALID_ARGUMENT),
+    (dict(scale=float("nan")), tla.ERR_INVALID_ARGUMENT), (dict(gqa_map=3), tla.ERR_INVALID_ARGUMENT)])
+def test_scaled_prefill_refuses_descriptors(kw, code):
+    assert _prefill(_prefill_desc(**kw)) == code
+    assert tla.last_error()
+
+
+def test_scaled_prefill_refuses_arguments():
+    d = _prefill_desc()
+    assert _prefill(None) == tla.ERR_INVALID_ARGUMENT
+    for name in ("out", "q", "cu", "k", "v", "ks", "vs", "bt", "sl"):
+        assert _prefill(d, **{name: None}) == tla.ERR_INVALID_ARGUMENT, name
+    for name in ("q", "k", "v", "ks", "vs", "out"):
+        assert _prefill(d, **{name: ctypes.c_void_p(0x1002)}) == tla.ERR_INVALID_ARGUMENT, name
+    assert _prefill(d, total=16, most=17) == tla.ERR_INVALID_ARGUMENT
+    assert _prefill(d, total=-1) == tla.ERR_INVALID_ARGUMENT
+    assert _prefill(d, total=0, most=0, out=None, q=None, ks=None, vs=None) == tla.OK
+
+
+def test_scaled_prefill_binding_refuses_wrong_tensors():
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    good = dict(q=torch.zeros(9, 8, 128, dtype=bf), out=torch.zeros(9, 8, 128, dtype=bf), cu=torch.zeros(4, dtype=i32),
+                k=torch.zeros(6, 2, 128, 16, dtype=u8), v=torch.zeros(6, 2, 128, 16, dtype=u8), ks=torch.zeros(6, 2, 16),
+                vs=torch.zeros(6, 2, 16), bt=torch.zeros(3, 5, dtype=i32), sl=torch.zeros(3, dtype=i32))
+    desc = tla.make_prefill_desc(good["q"], good["k"], good["bt"], 3, 2, 0.1, kv_dtype=tla.FP8_E4M3)
+    for kw in (dict(q=good["q"].half()), dict(out=good["out"][:8]), dict(q=good["q"][:, :4], out=good["out"][:, :4]),
+               dict(cu=good["cu"][:3]), dict(cu=good["cu"].long()), dict(k=good["k"][:5]), dict(ks=good["ks"].half()),
+               dict(vs=good["vs"][:, :, :8]), dict(bt=good["bt"][:2]), dict(sl=good["sl"].long()), dict()):
+        a = {**good, **kw}
+        with pytest.raises(tla.TLError):
+            tla.chunked_prefill_scaled(desc, a["out"], a["q"], a["cu"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["sl"], 4)

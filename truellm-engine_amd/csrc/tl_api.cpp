@@ -1390,9 +1390,10 @@ int32_t tl_kivi_pass_runs(int32_t seq_len, int32_t n_kv_heads, int32_t head_dim,
   return need <= scratch_bytes;
 }
 
-int tl_chunked_prefill(const tl_prefill_desc* d, void* out, const void* q, const int32_t* cu_q_lens,
-                       const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                       const int32_t* seq_lens, int32_t total_q, int32_t max_q_len, void* stream) {
+static int prefill_impl(const tl_prefill_desc* d, void* out, const void* q, const int32_t* cu_q_lens,
+                        const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                        const int32_t* seq_lens, int32_t total_q, int32_t max_q_len, void* stream,
+                        const float* k_scales, const float* v_scales) {
   if (!d) return fail(TL_ERR_INVALID_ARGUMENT, "desc is NULL");
   if (d->num_seqs < 0 || total_q < 0 || max_q_len < 0)
     return fail(TL_ERR_INVALID_ARGUMENT, "num_seqs=%d total_q=%d max_q_len=%d must be >= 0",
@@ -1447,12 +1448,37 @@ int tl_chunked_prefill(const tl_prefill_desc* d, void* out, const void* q, const
   a.gqa_map = d->gqa_map; a.max_q_len = max_q_len; a.scale = d->scale;
   a.k_scale = kv_dtype == TL_DTYPE_FP8_E4M3 ? d->k_scale : 1.f;
   a.v_scale = kv_dtype == TL_DTYPE_FP8_E4M3 ? d->v_scale : 1.f;
+  a.k_scales = k_scales; a.v_scales = v_scales;
   a.num_prefill_seqs = d->num_prefill_seqs;
   a.stream = (hipStream_t)stream;
   const int lrc = tl::launch_prefill(a);
   if (lrc == 3) return fail(TL_ERR_NOT_IMPLEMENTED, "no prefill kernel for block_size=%d", d->block_size);
   if (lrc) return fail(TL_ERR_BACKEND, "prefill launch failed");
   return ok();
+}
+
+int tl_chunked_prefill(const tl_prefill_desc* d, void* out, const void* q, const int32_t* cu_q_lens,
+                       const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                       const int32_t* seq_lens, int32_t total_q, int32_t max_q_len, void* stream) {
+  return prefill_impl(d, out, q, cu_q_lens, k_cache, v_cache, block_tables, seq_lens, total_q, max_q_len, stream,
+                      nullptr, nullptr);
+}
+
+int tl_chunked_prefill_scaled(const tl_prefill_desc* desc, void* out, const void* q, const int32_t* cu_q_lens,
+                              const void* k_cache, const void* v_cache, const float* k_scales,
+                              const float* v_scales, const int32_t* block_tables, const int32_t* seq_lens,
+                              int32_t total_q, int32_t max_q_len, void* stream) {
+  if (!desc) return fail(TL_ERR_INVALID_ARGUMENT, "desc is NULL");
+  if (desc->kv_dtype != TL_DTYPE_FP8_E4M3)
+    return fail(TL_ERR_INVALID_ARGUMENT, "kv_dtype=%d: scales of each token go with FP8_E4M3", desc->kv_dtype);
+  if (desc->num_seqs > 0 && total_q > 0) {
+    const int rc = check_scales(k_scales, v_scales, desc->head_size);
+    if (rc) return rc;
+  }
+  tl_prefill_desc d = *desc;
+  d.k_scale = d.v_scale = 1.f;
+  return prefill_impl(&d, out, q, cu_q_lens, k_cache, v_cache, block_tables, seq_lens, total_q, max_q_len, stream,
+                      k_scales, v_scales);
 }
 
 }  // extern "C"

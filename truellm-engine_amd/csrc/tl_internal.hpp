@@ -224,6 +224,8 @@ struct PrefillLaunch {
   int num_seqs, num_heads, num_kv_heads, block_size, max_blocks_per_seq, num_blocks;
   int dtype, gqa_map, max_q_len, num_prefill_seqs;
   int kv_dtype;                 // dtype, or FP8 E4M3 (k_scale, v_scale: the per-tensor scales)
+  const float* k_scales;        // FP8 with a scale for each token and kv head [N, n_kv, bs], else null
+  const float* v_scales;
   float scale, k_scale, v_scale;
   hipStream_t stream;
 };

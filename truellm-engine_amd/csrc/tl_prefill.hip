@@ -39,7 +39,12 @@
 // Pools: f16 / bf16 (the q type), or FP8 E4M3 with per-tensor k_scale /
 // v_scale (codes converted exactly to the q type for q.k and to f16 for
 // p.v as they are staged; k_scale folds into the score scale, v_scale into
-// the output).  Block sizes: any power of two 8 .. 256; a wavefront's 16-key
+// the output), or FP8 with a scale for each token and kv head (FP8S: both
+// scales reach the softmax through LDS; the key's multiplies its score, the
+// value's its weight before that is rounded to f16.  A power of two near the
+// largest value scale so far divides every weight and row sum, so that values
+// of any size keep f16's precision; it is carried as an addend of the
+// running maximum).  Block sizes: any power of two 8 .. 256; a wavefront's 16-key
 // group lies in one block from 16 on, in two at 8 (one per lane half; the
 // split kernel copies block by block there).
 //
@@ -148,6 +153,11 @@ struct PrefillSmem {
     float row[NW][kPfRows];                       // per-row exchange (alpha, l)
   } pf;
 };
+// FP8S: the scales of an iteration's keys and of their values (0 where there
+// is no token).  prefill_kernel keeps those of iteration i in row i % 4: they
+// are read by its softmax, two phases after K, when K's stage is written again.
+template <int ROWS> struct KeyScales { float k[ROWS][kPfKeys], v[ROWS][kPfKeys]; };
+template <> struct KeyScales<0> {};
 
 // A block-table row read through the constant address space: the table is
 // not written during the kernel, and with a wave-uniform index the reads
@@ -201,6 +211,37 @@ __device__ __forceinline__ u32x4 fp8x8_to(const u32x4& c) {
   return u32x4{cvt(c.x, false), cvt(c.x, true), cvt(c.y, false), cvt(c.y, true)};
 }
 
+// A lane's scores (or weights) of keys 32 t + 8 j + 4 g + i times their scales.
+template <class V>
+__device__ __forceinline__ void scale_keys(V& x, const float* of, int t, int g) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 k4 = *reinterpret_cast<const float4*>(of + 32 * t + 8 * j + 4 * g);
+    x[4 * j] *= k4.x;
+    x[4 * j + 1] *= k4.y;
+    x[4 * j + 2] *= k4.z;
+    x[4 * j + 3] *= k4.w;
+  }
+}
+// The unit that the value scales are taken in: 2^e, raised when a scale of the
+// iteration passes 2^6 of it (weights stay below 2^8, so below 2^14 with it).
+struct ValueUnit {
+  float unit = 0.f, e = 0.f;
+  // whether it has to be raised for the iteration's scales v (one a lane)
+  __device__ __forceinline__ bool passed(float v, float& top) const {
+    top = mw::max_kg(row_max(v));
+    return top > 64.f * unit;
+  }
+  // the factor of what was summed so far
+  __device__ __forceinline__ float raise(float top) {
+    const int x = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
+    const float f = __builtin_amdgcn_exp2f(e - (float)x);
+    e = (float)x;
+    unit = __builtin_bit_cast(float, (uint32_t)(x + 127) << 23);
+    return f;
+  }
+};
+
 // Decode rows (q_len == 1) of a mixed batch, one workgroup per (sequence,
 // kv head, 16-head slice), q / out row cu_q_lens[s]: the matrix-core decode
 // wavefronts (tl_mfma_wave.hpp), so a GQA group of up to 16 heads reads its
@@ -229,15 +270,18 @@ template <Kind Q, Kind KV, int BS, int NW, bool ROWS>
 __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
   static_assert(BS >= 8 && BS <= 256 && (BS & (BS - 1)) == 0, "block size: a power of two 8 .. 256");
   static_assert(NW == 8, "two groups of four wavefronts, one wavefront of each group per SIMD");
-  static_assert(KV == Q || KV == Kind::FP8, "a 2-byte pool holds the q type");
+  static_assert(KV == Q || is_fp8<KV>(), "a 2-byte pool holds the q type");
+  constexpr bool kScaled = KV == Kind::FP8S;
+  using Pv = PvScale<KV>;
   constexpr int BPI = BS >= kPfKeys ? 1 : kPfKeys / BS;   // pool blocks per iteration
   constexpr int BSE = BS >= kPfKeys ? kPfKeys : BS;       // keys of an iteration per block
   constexpr int NKE = BS == 8 ? 2 : 1;                    // blocks of a wavefront's 16-key group
-  constexpr int E = KV == Kind::FP8 ? 1 : 2;              // pool bytes per element
+  constexpr int E = is_fp8<KV>() ? 1 : 2;                 // pool bytes per element
   using M = Mfma32<Q>;                                 // q.k
   using MP = Mfma32<Kind::F16>;                        // p.v (f16 for every type)
   union Smem { PrefillSmem<NW> pf; DecodeRowSmem<ROWS ? NW : 1> dec; };
   __shared__ __attribute__((aligned(16))) Smem smem;
+  __shared__ __attribute__((aligned(16))) KeyScales<kScaled ? 4 : 0> key_scales;
   auto& sm = smem.pf;
   const int b0 = blockIdx.x;
   if constexpr (ROWS) {
@@ -324,7 +368,9 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
   // staged two phases ahead of its use, V one).  nv: keys of the lane's V
   // run that exist (the rest is zeroed when staged, so that the loads are
   // waited for only there).
-  struct Fetched { u32x4 k[kUnits], v[kUnits]; int nv; };
+  // FP8S: ks, vs are the scales of key kg + 8 (l >> 5) + (l & 7), both of K's
+  // iteration (a block holds a token's key and value).
+  struct Fetched { u32x4 k[kUnits], v[kUnits]; int nv; float ks, vs; };
   // unconditional loads (a missing block has an empty range and reads
   // zeros): no branch, so nothing waits for them before the staging
   auto rsrc_of = [&](const char* pool, int pb) {
@@ -357,6 +403,22 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
       return u32x4{a.x | b.x, a.y | b.y, a.z | b.z, a.w | b.w};
     }
   };
+  auto load_scale = [&](const float* scales, const int (&pb)[NKE], int it) -> float {
+    const int key = kg + 8 * g + (lane & 7);
+    const unsigned off = 4u * unsigned(BS > kPfKeys ? (int)((unsigned)(it * kPfKeys) % BS) + key : key % BS);
+    auto of = [&](int h) {
+      const int64_t row = pb[h] >= 0 ? ((int64_t)pb[h] * p.num_kv_heads + kvh) * BS : 0;
+      return buffer_rsrc(scales + row, pb[h] >= 0 ? 4u * BS : 0u);
+    };
+    if constexpr (NKE == 1) {
+      return __builtin_bit_cast(float, (unsigned)__builtin_amdgcn_raw_buffer_load_b32(of(0), off, 0, 0));
+    } else {
+      constexpr unsigned kPast = 0x40000000u;
+      const unsigned a = __builtin_amdgcn_raw_buffer_load_b32(of(0), g == 0 ? off : kPast, 0, 0);
+      const unsigned b = __builtin_amdgcn_raw_buffer_load_b32(of(NKE - 1), g == 1 ? off : kPast, 0, 0);
+      return __builtin_bit_cast(float, a | b);
+    }
+  };
   // physical block of half h of the wavefront's key group in iteration it
   // from its table entry, or -1
   auto group_block = [&](int it, int entry, int h) {
@@ -384,6 +446,10 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
   auto load = [&](const FetchPlan& fp, int i, Fetched& f) {
     if (i < kUnits) f.k[i] = load_unit(kpool, fp.pk, fp.it_k, unit_ch(i));
     else f.v[i - kUnits] = load_unit(vpool, fp.pv, fp.it_v, unit_ch(i - kUnits));
+    if constexpr (kScaled) {
+      if (i == 0) f.ks = load_scale(p.k_scales, fp.pk, fp.it_k);
+      if (i == 1) f.vs = load_scale(p.v_scales, fp.pk, fp.it_k);
+    }
   };
   auto fetch = [&](int it_k, int it_v, const Entries& e, Fetched& f) {
     const FetchPlan fp = plan(it_k, it_v, e, f);
@@ -391,15 +457,22 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
     for (int i = 0; i < 2 * kUnits; ++i) load(fp, i, f);
   };
   auto stage = [&](int it_k, int it_v, const Fetched& f) {
+    if constexpr (kScaled) {
+      if ((wave & 1) == 0 && c32 < 8) {
+        key_scales.k[it_k & 3][tok + c32] = f.ks;
+        // past the sequence's end a scale may be anything
+        key_scales.v[it_k & 3][tok + c32] = it_k * kPfKeys + tok + c32 < L ? f.vs : 0.f;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       // K as it lies in the pool: the lane's 8 keys of its channel, one
       // 16-byte write (k_operand reads it transposed)
-      const u32x4 kq = KV == Kind::FP8 ? fp8x8_to<Q>(f.k[u]) : f.k[u];
+      const u32x4 kq = is_fp8<KV>() ? fp8x8_to<Q>(f.k[u]) : f.k[u];
       *reinterpret_cast<u32x4*>(&sm.pf.kt[it_k & 1][unit_ch(u) * kKtStride + tok]) = kq;
       // V slots at or past the sequence end may hold anything (NaN codes
       // too, and a zero weight times NaN is NaN): zero them
-      u4v v = __builtin_bit_cast(u4v, KV == Kind::FP8 ? fp8x8_to<Kind::F16>(f.v[u]) : f.v[u]);
+      u4v v = __builtin_bit_cast(u4v, is_fp8<KV>() ? fp8x8_to<Kind::F16>(f.v[u]) : f.v[u]);
       const int nv = f.nv;
       // a wave-uniform branch (the sequence's last iteration only): as a
       // lane-divergent one it became selects run on every iteration
@@ -448,6 +521,7 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) o[c] = f16v{};
   float m_used = -INFINITY, l_part = 0.f;
+  ValueUnit v_unit;                                    // FP8S
   float* s_row = &sm.pf.row[wave][0];
   // Scores and weights of an iteration share registers: QK leaves the S^T
   // tiles in sp (MFMA phase), SM turns tile t into its packed f16 weights
@@ -499,6 +573,13 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
   auto softmax = [&](int it, int t_entries, auto mask_tag) {
     constexpr bool MASK = decltype(mask_tag)::value;
     const int k0 = it * kPfKeys;
+    float v_top = 0.f;
+    bool v_up = false;
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) scale_keys(sp[t], key_scales.k[it & 3], t, g);
+      v_up = v_unit.passed(key_scales.v[it & 3][lane], v_top);
+    }
     float mx = -INFINITY;
     if constexpr (!MASK) {
 #pragma unroll
@@ -528,9 +609,10 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
     }
     mx *= p.qk_scale;
     const bool raise = mx > m_used + kLazyRescale || (m_used == -INFINITY && mx != -INFINITY);
-    if (__builtin_amdgcn_ballot_w64(raise)) {
+    if (__builtin_amdgcn_ballot_w64(raise) || (kScaled && v_up)) {
       const float m_new = raise ? mx : m_used;
-      const float alpha = (m_new == m_used) ? 1.f : (m_used == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_used - m_new));
+      float alpha = (m_new == m_used) ? 1.f : (m_used == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_used - m_new));
+      if (kScaled && v_up) alpha *= v_unit.raise(v_top);
       m_used = m_new;
       l_part *= alpha;
       if (g == 0) s_row[c32] = alpha;
@@ -551,7 +633,8 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
     }
     // the weights carry 2^kPExp (see PvScale): a factor common to every
     // weight and row sum, so the rounding of m_use - kPExp cancels
-    const float m_use = ((m_used == -INFINITY) ? 0.f : m_used) - (float)PvScale<KV>::kPExp;
+    float m_use = ((m_used == -INFINITY) ? 0.f : m_used) - (float)Pv::kPExp;
+    if constexpr (kScaled) m_use += v_unit.e;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       float pw[16], ls[4] = {0.f, 0.f, 0.f, 0.f};
@@ -561,6 +644,7 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
         ls[r & 3] += pw[r];
       }
       l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      if constexpr (kScaled) scale_keys(pw, key_scales.v[it & 3], t, g);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const int r0 = 8 * s2;
@@ -763,7 +847,7 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float l = s_row[8 * j + 4 * g + i];
-      inv[i] = l > 0.f ? PvScale<KV>::kP * __builtin_amdgcn_rcpf(l) : 0.f;   // the sums carry 2^kPExp
+      inv[i] = l > 0.f ? Pv::kP * __builtin_amdgcn_rcpf(l) : 0.f;   // the sums carry 2^kPExp
       if constexpr (KV == Kind::FP8) inv[i] *= p.v_scale;
     }
 #pragma unroll
@@ -829,15 +913,18 @@ struct PrefillSplitSmem {
 template <Kind Q, Kind KV, int BS, bool ROWS>
 __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(PrefillParams pp) {
   static_assert(BS >= 8 && BS <= 256 && (BS & (BS - 1)) == 0, "block size: a power of two 8 .. 256");
-  static_assert(KV == Q || KV == Kind::FP8, "a 2-byte pool holds the q type");
+  static_assert(KV == Q || is_fp8<KV>(), "a 2-byte pool holds the q type");
+  constexpr bool kScaled = KV == Kind::FP8S;
+  using Pv = PvScale<KV>;
   constexpr int BSE = BS >= kPfKeys ? kPfKeys : BS;       // keys of an iteration per block
   constexpr int BPI = kPfKeys / BSE;                      // pool blocks per iteration
   constexpr int KR = BS == 8 ? 8 : 16;                    // keys of a staging run, which lies in one block
-  constexpr int E = KV == Kind::FP8 ? 1 : 2;              // pool bytes per element
+  constexpr int E = is_fp8<KV>() ? 1 : 2;                 // pool bytes per element
   using M = Mfma32<Q>;                                 // q.k
   using MP = Mfma32<Kind::F16>;                        // p.v (f16 for every type)
   union Smem { PrefillSplitSmem pf; DecodeRowSmem<ROWS ? kSplitNW : 1> dec; };
   __shared__ __attribute__((aligned(16))) Smem smem;
+  __shared__ __attribute__((aligned(16))) KeyScales<kScaled ? kSplit : 0> key_scales;   // a row for each key group
   auto& sm = smem.pf;
   const int b0 = blockIdx.x;
   if constexpr (ROWS) {
@@ -896,7 +983,8 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
   // prompts of 32 of 128 19.2, 11.8 (13.8).
   constexpr int kUnitCh = 8 * kWave / KR, kRuns = kPfKeys / KR / kSplitWaves, kUnits = kPfHead / kUnitCh;
   const int lane_ch = lane % kUnitCh, lane_tok = KR == 8 ? 0 : 8 * g;
-  struct Fetched { u32x4 k[kRuns][kUnits], v[kRuns][kUnits]; int nv[kRuns]; };
+  // FP8S: ks, vs are the scales of key lane_tok + (l & 7) of the run.
+  struct Fetched { u32x4 k[kRuns][kUnits], v[kRuns][kUnits]; int nv[kRuns]; float ks[kRuns], vs[kRuns]; };
   const int64_t head_bytes = (int64_t)kPfHead * BS * E;
   auto rsrc_of = [&](const char* pool, int pb) {
     const int64_t row = ((int64_t)max(pb, 0) * p.num_kv_heads + kvh) * head_bytes;
@@ -923,6 +1011,12 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
       for (int u = 0; u < kUnits; ++u)
         (PART == 0 ? f.k : f.v)[r][u] = load_raw(rsrc_of(PART == 0 ? p.k_cache : p.v_cache, pb),
                                                  unsigned(E * ((kUnitCh * u + lane_ch) * BS + in_blk)));
+      if constexpr (kScaled) {
+        const int64_t row = ((int64_t)max(pb, 0) * p.num_kv_heads + kvh) * BS;
+        const auto of = buffer_rsrc((PART == 0 ? p.k_scales : p.v_scales) + row, pb >= 0 ? 4u * BS : 0u);
+        (PART == 0 ? f.ks : f.vs)[r] = __builtin_bit_cast(
+            float, (unsigned)__builtin_amdgcn_raw_buffer_load_b32(of, 4u * unsigned(in_blk + (lane & 7)), 0, 0));
+      }
     }
   };
   const std::integral_constant<int, 0> kKeys;
@@ -934,7 +1028,13 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
         *reinterpret_cast<u32x4*>(&sm.st.kt[grp][(kUnitCh * u + lane_ch) * kKtStride + tok]) =
-            KV == Kind::FP8 ? fp8x8_to<Q>(f.k[r][u]) : f.k[r][u];
+            is_fp8<KV>() ? fp8x8_to<Q>(f.k[r][u]) : f.k[r][u];
+      if constexpr (kScaled) {
+        if (lane % (KR == 8 ? kWave : 32) < 8) {
+          key_scales.k[grp][tok + (lane & 7)] = f.ks[r];
+          key_scales.v[grp][tok + (lane & 7)] = (lane & 7) < f.nv[r] ? f.vs[r] : 0.f;   // past the end: anything
+        }
+      }
     }
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
@@ -943,7 +1043,7 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
       for (int u = 0; u < kUnits; ++u) {
         const int ch = kUnitCh * u + lane_ch;
         // V slots at or past the sequence end may hold anything: zero them
-        u4v v = __builtin_bit_cast(u4v, KV == Kind::FP8 ? fp8x8_to<Kind::F16>(f.v[r][u]) : f.v[r][u]);
+        u4v v = __builtin_bit_cast(u4v, is_fp8<KV>() ? fp8x8_to<Kind::F16>(f.v[r][u]) : f.v[r][u]);
         const int nv = f.nv[r];
         if (__builtin_amdgcn_ballot_w64(nv < 8)) {
 #pragma unroll
@@ -985,6 +1085,7 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
 #pragma unroll
   for (int c = 0; c < 4; ++c) o[c] = f16v{};
   float m_used = -INFINITY, l_part = 0.f;
+  ValueUnit v_unit;                                    // FP8S
   float* s_row = &sm.row[wave][0];
   auto wave_sync = [&]() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -1040,6 +1141,13 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
       for (int t = 0; t < KT; ++t) sp[t] = M::mma(kb[ks % (kAhead + 1)][t], qb[ks], sp[t]);
     }
     after_scores();
+    float v_top = 0.f;
+    bool v_up = false;
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) scale_keys(sp[t], key_scales.k[grp], t, g);
+      v_up = v_unit.passed(key_scales.v[grp][lane], v_top);
+    }
     bool blk_ok[BPI], all_ok = k0 + kPfKeys - 1 <= wmin_pos;
 #pragma unroll
     for (int i = 0; i < BPI; ++i) {
@@ -1067,14 +1175,16 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
     }
     mx *= p.qk_scale;
     const bool raise = mx > m_used + kLazyRescale || (m_used == -INFINITY && mx != -INFINITY);
-    if (__builtin_amdgcn_ballot_w64(raise)) {
+    if (__builtin_amdgcn_ballot_w64(raise) || (kScaled && v_up)) {
       const float m_new = raise ? mx : m_used;
-      const float alpha = (m_new == m_used) ? 1.f : (m_used == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_used - m_new));
+      float alpha = (m_new == m_used) ? 1.f : (m_used == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_used - m_new));
+      if (kScaled && v_up) alpha *= v_unit.raise(v_top);
       m_used = m_new;
       l_part *= alpha;
       scale_rows(alpha);
     }
-    const float m_use = ((m_used == -INFINITY) ? 0.f : m_used) - (float)PvScale<KV>::kPExp;
+    float m_use = ((m_used == -INFINITY) ? 0.f : m_used) - (float)Pv::kPExp;
+    if constexpr (kScaled) m_use += v_unit.e;
     u32x4 pa[KT][2];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -1085,6 +1195,7 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
         ls[r & 3] += pw[r];
       }
       l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      if constexpr (kScaled) scale_keys(pw, key_scales.v[grp], t, g);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2)
         pa[t][s2] = u32x4{MP::pack(pw[8 * s2], pw[8 * s2 + 1]), MP::pack(pw[8 * s2 + 2], pw[8 * s2 + 3]),
@@ -1109,7 +1220,7 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
     return __builtin_bit_cast(float, (unsigned)sw[0]) + __builtin_bit_cast(float, (unsigned)sw[1]);
   };
   // factor of a row of the output (the sums carry 2^kPExp)
-  auto row_inverse = [&](float l) { return l > 0.f ? PvScale<KV>::kP * __builtin_amdgcn_rcpf(l) : 0.f; };
+  auto row_inverse = [&](float l) { return l > 0.f ? Pv::kP * __builtin_amdgcn_rcpf(l) : 0.f; };
   const float rg = 1.f / (float)p.group;               // rows of the output as in prefill_kernel
   const int64_t obase = (int64_t)q0 * p.num_heads + (p.gqa_map ? kvh * p.group : kvh);
   const int rmul = p.gqa_map ? 1 : p.num_kv_heads, qmul = p.gqa_map ? p.num_heads - p.group : 0;
@@ -1162,6 +1273,8 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
   }
 
   const float l = row_sum();
+  // the groups' units join their maxima: a weight is in 2^(m_used + e)
+  if constexpr (kScaled) m_used += v_unit.e;
   // One iteration (a prompt's first 64 keys): group 0 has the sums, nothing
   // to merge.  bf16, 16 queries of 16 keys 8.1 us, 64 of 64 8.3 (through the
   // merge 10.5 and 10.6, prefill_kernel 9.1 and 10.9).
@@ -1305,6 +1418,7 @@ int launch_prefill(const PrefillLaunch& a) {
   // v_scale the output
   p.qk_scale = a.scale * (fp8 ? a.k_scale : 1.f) * kLog2e;
   p.v_scale = fp8 ? a.v_scale : 1.f;
+  p.k_scales = a.k_scales; p.v_scales = a.v_scales;
   p.block_size = a.block_size;
   pp.cu_q_lens = a.cu_q_lens;
   pp.num_seqs = a.num_seqs;
@@ -1319,6 +1433,9 @@ int launch_prefill(const PrefillLaunch& a) {
   const unsigned grid = (unsigned)(pp.row_tiles * pp.pf_seqs * a.num_kv_heads);
   pp.pf_wgs = (int)grid;
   const bool bf16 = a.dtype == (int)Kind::BF16;
+  if (fp8 && a.k_scales)
+    return bf16 ? launch_prefill_bs<Kind::BF16, Kind::FP8S>(pp, a.block_size, grid, a.stream)
+                : launch_prefill_bs<Kind::F16, Kind::FP8S>(pp, a.block_size, grid, a.stream);
   if (fp8)
     return bf16 ? launch_prefill_bs<Kind::BF16, Kind::FP8>(pp, a.block_size, grid, a.stream)
                 : launch_prefill_bs<Kind::F16, Kind::FP8>(pp, a.block_size, grid, a.stream);

@@ -181,6 +181,7 @@ _SIG = {
     "tl_kivi_pass_params": (ctypes.c_int, [_I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "tl_kivi_pass_runs": (_I, [_I, _I, _I, _I, _I, ctypes.c_size_t]),
     "tl_chunked_prefill": (ctypes.c_int, [ctypes.POINTER(PrefillDesc), _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "tl_chunked_prefill_scaled": (ctypes.c_int, [ctypes.POINTER(PrefillDesc)] + [_P] * 9 + [_I, _I, _P]),
     "tl_kivi_paged_attention_decode": (ctypes.c_int, [ctypes.POINTER(KiviDesc), _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, ctypes.c_size_t, _P]),
     "tl_kivi_rope_step_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(KiviDesc), _I]),
     "tl_kivi_rope_decode_step": (ctypes.c_int, [ctypes.POINTER(KiviDesc)] + [_P] * 7 + [_I, _I] + [_P] * 7
@@ -830,6 +831,26 @@ def chunked_prefill(desc, out, q, cu_q_lens, k_cache, v_cache, block_tables, seq
     check(lib.tl_chunked_prefill(ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(cu_q_lens),
                                  _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(seq_lens),
                                  q.shape[0], max_q_len, _stream(stream)))
+
+
+def chunked_prefill_scaled(desc, out, q, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
+                           max_q_len, stream=None):
+    """chunked_prefill over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
+    S = desc.num_seqs
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, desc.num_kv_heads, desc.head_size,
+                 desc.block_size)
+    _check_ints(cu_q_lens, (S + 1,), "cu_q_lens")
+    _check_ints(block_tables, (S, desc.max_blocks_per_seq), "block_tables")
+    _check_ints(seq_lens, (S,), "seq_lens")
+    for t in (q, out):
+        if t.shape != (q.shape[0], desc.num_heads, desc.head_size) or dtype_code(t) != desc.dtype \
+                or not t.is_contiguous():
+            raise TLError(ERR_INVALID_ARGUMENT, f"q / out {tuple(t.shape)} {t.dtype}: contiguous [total_q, "
+                          f"{desc.num_heads}, {desc.head_size}] of the descriptor's type")
+    _on_gpu(q, out, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens)
+    check(lib.tl_chunked_prefill_scaled(
+        ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(cu_q_lens), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+        _ptr(v_scales), _ptr(block_tables), _ptr(seq_lens), q.shape[0], max_q_len, _stream(stream)))
 
 
 # ---------------------------------------------------------------------------
