@@ -226,6 +226,23 @@ __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
 
+// Lane N of the lane's row of 16, all of them active, as an operand of the
+// instruction that uses it (which the compiler folds only with bound_ctrl set).
+template <int N>
+__device__ __forceinline__ float row_lane(float v) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kDppLane0 + N, 0xF, 0xF, true));
+}
+
+// x times lane N's y.  Opaque: two products that are packed together become a
+// vector operation otherwise, whose operands are registers of their own.
+template <int N>
+__device__ __forceinline__ float mul_row_lane(float x, float y) {
+  float r = x * row_lane<N>(y);
+  asm("" : "+v"(r));
+  return r;
+}
+
 // Max / sum over the 16 lanes of a row (masks 1, 2, 7, 15 span the 4 bits).
 __device__ __forceinline__ float row_max(float v) {
   v = __builtin_fmaxf(v, dpp<kDppXor1>(v));

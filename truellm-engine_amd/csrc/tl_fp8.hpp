@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 // A lane's bits of another lane of its row of 16 (a DPP control of tl_device.hpp).
 template <int CTRL>
 __device__ __forceinline__ uint32_t lane_bits(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false);
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
 __device__ __forceinline__ uint32_t lanes_umax_16(uint32_t v) {   // with lane ^ 16
   const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);

@@ -25,8 +25,11 @@
 
 #include "tl_decode_wave.hpp"
 #include "tl_device.hpp"
+#include "tl_fp8.hpp"
 
 #include <math.h>
+
+#include <utility>
 
 namespace tl {
 namespace mw {
@@ -186,13 +189,13 @@ __device__ __forceinline__ u32x4 keep_halves(const u32x4& v, int n) {
 // each token).
 struct State {
   f4 o[8];
-  float m_run, l_lane, unit;
+  float m_run, l_lane, unit, inv_unit;
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = f4{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
     l_lane = 0.f;
-    unit = 1.f;
+    unit = inv_unit = 1.f;
   }
   // Raises the running max to the wavefront's new max mx when it grew by
   // more than 2^8 for some head.
@@ -206,18 +209,19 @@ struct State {
       m_run = m_new;
     }
   }
-  // Scales of values in a unit near the largest of them (v: this lane's token
-  // of the iteration): returns 1 / unit.
-  __device__ __forceinline__ float raise_unit(float v) {
-    const float top = max_kg(row_max(v));
-    if (top > 64.f * unit) {                           // the same in every lane; also where unit is 0
-      const float u = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, top) & 0x7f800000u);
-      const float f = unit / u;
+  // Scales of values are taken in a unit near the largest of them so far.
+  __device__ __forceinline__ void no_unit() { unit = inv_unit = 0.f; }
+  // v: that of this lane's token of the iteration
+  __device__ __forceinline__ void raise_unit(float v) {
+    const float top = __builtin_bit_cast(float, lanes_umax<kWave>(__builtin_bit_cast(uint32_t, v)));
+    if (__builtin_amdgcn_ballot_w64(top > 64.f * unit) != 0) {   // the same in every lane; also where unit is 0
+      const uint32_t e = min(__builtin_bit_cast(uint32_t, top) >> 23, 252u);   // 2^125 at most: its inverse is normal
+      const float u = __builtin_bit_cast(float, e << 23), f = unit * __builtin_bit_cast(float, (254u - e) << 23);
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
       unit = u;
+      inv_unit = __builtin_bit_cast(float, (254u - e) << 23);
     }
-    return unit > 0.f ? 1.f / unit : 0.f;
   }
   __device__ __forceinline__ void store(float v_scale, int m, int kg, float* s_acc_w, float* s_m_w,
                                         float* s_l_w) const {
@@ -242,19 +246,13 @@ struct NoFlush {
 };
 
 // s[i][r] times x of lane 4 r + i of the row (the token whose score it is).
-template <int N>
-__device__ __forceinline__ float row_lane(float x) { return dpp<kDppLane0 + N>(x); }
-__device__ __forceinline__ void scale_scores(f4 (&s)[4], float x) {
-  s[0][0] *= row_lane<0>(x);  s[1][0] *= row_lane<1>(x);  s[2][0] *= row_lane<2>(x);  s[3][0] *= row_lane<3>(x);
-  s[0][1] *= row_lane<4>(x);  s[1][1] *= row_lane<5>(x);  s[2][1] *= row_lane<6>(x);  s[3][1] *= row_lane<7>(x);
-  s[0][2] *= row_lane<8>(x);  s[1][2] *= row_lane<9>(x);  s[2][2] *= row_lane<10>(x); s[3][2] *= row_lane<11>(x);
-  s[0][3] *= row_lane<12>(x); s[1][3] *= row_lane<13>(x); s[2][3] *= row_lane<14>(x); s[3][3] *= row_lane<15>(x);
+template <class V, int... N>
+__device__ __forceinline__ void scale_tokens(V& s, float x, std::integer_sequence<int, N...>) {
+  ((s[N % 4][N / 4] = mul_row_lane<N>(s[N % 4][N / 4], x)), ...);
 }
-__device__ __forceinline__ void scale_weights(float (&w)[4][4], float x) {
-  w[0][0] *= row_lane<0>(x);  w[1][0] *= row_lane<1>(x);  w[2][0] *= row_lane<2>(x);  w[3][0] *= row_lane<3>(x);
-  w[0][1] *= row_lane<4>(x);  w[1][1] *= row_lane<5>(x);  w[2][1] *= row_lane<6>(x);  w[3][1] *= row_lane<7>(x);
-  w[0][2] *= row_lane<8>(x);  w[1][2] *= row_lane<9>(x);  w[2][2] *= row_lane<10>(x); w[3][2] *= row_lane<11>(x);
-  w[0][3] *= row_lane<12>(x); w[1][3] *= row_lane<13>(x); w[2][3] *= row_lane<14>(x); w[3][3] *= row_lane<15>(x);
+template <class V>
+__device__ __forceinline__ void scale_tokens(V& s, float x) {
+  scale_tokens(s, x, std::make_integer_sequence<int, 16>());
 }
 
 // ---- FP8 E4M3 KV, f16 / bf16 q: 64 tokens per iteration ----
@@ -395,11 +393,24 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
   // the scale of iteration token `lane`, in the iteration of entries b (a
   // missing block reads block 0, as the loads above)
   const int sb = NB > 1 ? lane / BS : 0, st_off = NB > 1 ? lane % BS : lane;
-  auto scale_at = [&](const float* scales, const Blocks<NB>& b, int ib) {
-    return scales[((int64_t)max(pick(b, sb), 0) * p.num_kv_heads + kvh) * BS + st_off + ib];
+  // (opaque selects: as in pick the compiler makes branches of them, twice
+  // an iteration)
+  auto scale_block = [&](const Blocks<NB>& b) {
+    int e = b.e[0];
+#pragma unroll
+    for (int i = 1; i < NB; ++i) {
+      e = sb >= i ? b.e[i] : e;
+      asm volatile("" : "+v"(e));
+    }
+    return e;
+  };
+  auto load_scales = [&](const Blocks<NB>& b, int ib, float& k, float& v) {
+    const int64_t at = ((int64_t)max(scale_block(b), 0) * p.num_kv_heads + kvh) * BS + st_off + ib;
+    k = p.k_scales[at];
+    v = p.v_scales[at];
   };
   float ks = 0.f, vs = 0.f;
-  if constexpr (kScaled) st.unit = 0.f;               // none seen
+  if constexpr (kScaled) st.no_unit();
 
   int it = first_it;
   Blocks<NB> cur = table_blocks<NB, BS>(p, table, it, t1);
@@ -412,8 +423,7 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
     const int ib = in_block_bytes<BS, TPI, 1>(it);
     load_k(kw, kbase0 + ib + (int64_t)max(pick(cur, kb), 0) * pool_stride);
     if constexpr (kScaled) {
-      ks = scale_at(p.k_scales, cur, ib);
-      vs = scale_at(p.v_scales, cur, ib);
+      load_scales(cur, ib, ks, vs);
     }
     __builtin_amdgcn_sched_barrier(0);
     load_v(vr, v_at(cur, ib, vb), v_at(cur, ib, vb2));
@@ -425,7 +435,7 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       if (it != first_it && it % flush.part_tokens == 0) {   // a partition ends: its partials out, state afresh
         flush(st, it / flush.part_tokens - 1);
         st.init();
-        if constexpr (kScaled) st.unit = 0.f;
+        if constexpr (kScaled) st.no_unit();
       }
     }
     const Blocks<NB> nn = table_blocks<NB, BS>(p, table, it + 2 * step, t1);
@@ -479,7 +489,7 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
     }
     auto tok_ok = [&](int t) { return kSplitRun ? ((keep >> t) & 1u) != 0 : t < n_ok; };
     // (bf16: qk_scale is the head's, not the token's, and stays with the lane)
-    if constexpr (kScaled) scale_scores(s, QK == Kind::BF16 ? ks : ks * qk_scale);
+    if constexpr (kScaled) scale_tokens(s, QK == Kind::BF16 ? ks : ks * qk_scale);
     float sc[4][4];
     float mx = -INFINITY;
 #pragma unroll
@@ -500,12 +510,11 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       }
     if constexpr (kScaled) {
       // the lane's own token: past the end or in a hole its scale may be anything
-      const float v_own = pick(cur, sb) >= 0 && it + lane < t1 ? vs : 0.f;
-      const float inv = st.raise_unit(v_own);
-      scale_weights(pw, v_own * inv);
+      const float v_own = scale_block(cur) >= 0 && it + lane < t1 ? vs : 0.f;
+      st.raise_unit(v_own);
+      scale_tokens(pw, v_own * st.inv_unit);
       // the next iteration's, after this one's last use of the registers
-      ks = scale_at(p.k_scales, nxt, ib_next);
-      vs = scale_at(p.v_scales, nxt, ib_next);
+      load_scales(nxt, ib_next, ks, vs);
     }
     // P^T operands: MFMA h takes tokens 8 h .. 8 h + 7 = (r = 2 h, 2 h + 1) x (i = 0 .. 3).
     // Where out is f16 (kLow) the rest that rounding a weight to f16 leaves

@@ -51,8 +51,11 @@
 // Nearest reference analogues: the per-token prefill of cuda_engine.cpp:842-860
 // and the dense attention of megakernel.cu:267-351; the reference has no
 // chunked prefill over the paged pool.
+#include <utility>
+
 #include "tl_decode_wave.hpp"
 #include "tl_device.hpp"
+#include "tl_fp8.hpp"
 #include "tl_internal.hpp"
 #include "tl_mfma_wave.hpp"
 
@@ -211,26 +214,33 @@ __device__ __forceinline__ u32x4 fp8x8_to(const u32x4& c) {
   return u32x4{cvt(c.x, false), cvt(c.x, true), cvt(c.y, false), cvt(c.y, true)};
 }
 
-// A lane's scores (or weights) of keys 32 t + 8 j + 4 g + i times their scales.
+// The scales of an S^T tile for its scores: value r of a lane is key 8 (r >> 2)
+// + 4 g + (r & 3) of the tile, so lane n of each row of 16 holds that of value
+// n, and the row's lanes take it by a broadcast (DPP, an operand of the
+// multiply): one 4-byte read of LDS a tile.  8 x 512 tokens of 2048, 64 heads:
+// 326 us; with the scales read as four 16-byte vectors a tile 351, with the
+// broadcasts as instructions of their own 327 and the whole call with its
+// decode rows 361 in place of 349 (without scales 300 and 327).
+__device__ __forceinline__ float tile_scales(const float* of, int t, int lane) {
+  return of[32 * t + 8 * ((lane >> 2) & 3) + 4 * (lane >> 5) + (lane & 3)];
+}
+template <class V, int... R>
+__device__ __forceinline__ void scale_row(V& x, float of, std::integer_sequence<int, R...>) {
+  ((x[R] = mul_row_lane<R>(x[R], of)), ...);
+}
 template <class V>
-__device__ __forceinline__ void scale_keys(V& x, const float* of, int t, int g) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float4 k4 = *reinterpret_cast<const float4*>(of + 32 * t + 8 * j + 4 * g);
-    x[4 * j] *= k4.x;
-    x[4 * j + 1] *= k4.y;
-    x[4 * j + 2] *= k4.z;
-    x[4 * j + 3] *= k4.w;
-  }
+__device__ __forceinline__ void scale_keys(V& x, float of) {
+  scale_row(x, of, std::make_integer_sequence<int, 16>());
 }
 // The unit that the value scales are taken in: 2^e, raised when a scale of the
 // iteration passes 2^6 of it (weights stay below 2^8, so below 2^14 with it).
 struct ValueUnit {
   float unit = 0.f, e = 0.f;
-  // whether it has to be raised for the iteration's scales v (one a lane)
+  // whether it has to be raised for the iteration's scales v (the same ones on
+  // the rows of a lane half)
   __device__ __forceinline__ bool passed(float v, float& top) const {
-    top = mw::max_kg(row_max(v));
-    return top > 64.f * unit;
+    top = __builtin_bit_cast(float, lanes_umax_32(lanes_umax<16>(__builtin_bit_cast(uint32_t, v))));
+    return __builtin_amdgcn_ballot_w64(top > 64.f * unit) != 0;
   }
   // the factor of what was summed so far
   __device__ __forceinline__ float raise(float top) {
@@ -573,12 +583,18 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
   auto softmax = [&](int it, int t_entries, auto mask_tag) {
     constexpr bool MASK = decltype(mask_tag)::value;
     const int k0 = it * kPfKeys;
-    float v_top = 0.f;
+    float v_top = 0.f, v_of[KT];
     bool v_up = false;
     if constexpr (kScaled) {
+      float k_of[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) scale_keys(sp[t], key_scales.k[it & 3], t, g);
-      v_up = v_unit.passed(key_scales.v[it & 3][lane], v_top);
+      for (int t = 0; t < KT; ++t) {
+        k_of[t] = tile_scales(key_scales.k[it & 3], t, lane);
+        v_of[t] = tile_scales(key_scales.v[it & 3], t, lane);
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) scale_keys(sp[t], k_of[t]);
+      v_up = v_unit.passed(fmaxf(v_of[0], v_of[1]), v_top);
     }
     float mx = -INFINITY;
     if constexpr (!MASK) {
@@ -644,7 +660,7 @@ __global__ __launch_bounds__(NW * kWave) void prefill_kernel(PrefillParams pp) {
         ls[r & 3] += pw[r];
       }
       l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      if constexpr (kScaled) scale_keys(pw, key_scales.v[it & 3], t, g);
+      if constexpr (kScaled) scale_keys(pw, v_of[t]);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const int r0 = 8 * s2;
@@ -1141,12 +1157,18 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
       for (int t = 0; t < KT; ++t) sp[t] = M::mma(kb[ks % (kAhead + 1)][t], qb[ks], sp[t]);
     }
     after_scores();
-    float v_top = 0.f;
+    float v_top = 0.f, v_of[KT];
     bool v_up = false;
     if constexpr (kScaled) {
+      float k_of[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) scale_keys(sp[t], key_scales.k[grp], t, g);
-      v_up = v_unit.passed(key_scales.v[grp][lane], v_top);
+      for (int t = 0; t < KT; ++t) {
+        k_of[t] = tile_scales(key_scales.k[grp], t, lane);
+        v_of[t] = tile_scales(key_scales.v[grp], t, lane);
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) scale_keys(sp[t], k_of[t]);
+      v_up = v_unit.passed(fmaxf(v_of[0], v_of[1]), v_top);
     }
     bool blk_ok[BPI], all_ok = k0 + kPfKeys - 1 <= wmin_pos;
 #pragma unroll
@@ -1195,7 +1217,7 @@ __global__ __launch_bounds__(kSplitNW * kWave) void prefill_split_kernel(Prefill
         ls[r & 3] += pw[r];
       }
       l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      if constexpr (kScaled) scale_keys(pw, key_scales.v[grp], t, g);
+      if constexpr (kScaled) scale_keys(pw, v_of[t]);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2)
         pa[t][s2] = u32x4{MP::pack(pw[8 * s2], pw[8 * s2 + 1]), MP::pack(pw[8 * s2 + 2], pw[8 * s2 + 3]),
