@@ -6,6 +6,7 @@
 #include "tl_device.hpp"
 #include "tl_fp8.hpp"
 #include "tl_internal.hpp"
+#include "tl_row.hpp"
 
 namespace tl {
 
@@ -77,14 +78,43 @@ struct TileAppend {
   uint32_t axis_of[8];                     // 2 bits for each rotation pair
 };
 
-// AXES: whether token t is at a place of the tables on every axis.
-__device__ __forceinline__ bool placed(const TileAppend& a, int64_t t) {
-  bool in = true;
-  for (int x = 0; x < a.num_axes; ++x) {
-    const int pos = a.positions[x * (int64_t)a.num_tokens + t];
-    in = in && pos >= 0 && pos < a.max_positions;
+// AXES: token t's position on each axis, all read at once (the last one again
+// past num_axes), and whether every one is a row of the tables.
+struct alignas(16) Places {
+  int pos[4];
+  Places() = default;
+  __device__ __forceinline__ Places(const TileAppend& a, int64_t t) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) pos[x] = a.positions[min(x, a.num_axes - 1) * (int64_t)a.num_tokens + t];
   }
-  return in;
+  __device__ __forceinline__ bool in_tables(const TileAppend& a) const {
+    bool in = true;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) in &= (unsigned)pos[x] < (unsigned)a.max_positions;   // no branch between the reads
+    return in;
+  }
+  // (Opaque selects here and below, or the compiler makes an indexed read of a
+  // copy in LDS or scratch of them.)
+  __device__ __forceinline__ int on(uint32_t axis) const {
+    int r = pos[0];
+#pragma unroll
+    for (int x = 1; x < 4; ++x) {
+      r = axis == (uint32_t)x ? pos[x] : r;
+      asm("" : "+v"(r));
+    }
+    return r;
+  }
+};
+// The axes of pairs 16 w .. 16 w + 15, 2 bits each, by selects: an indexed
+// read of the arguments is a round trip to memory before the tables' own.
+__device__ __forceinline__ uint32_t axes_word(const TileAppend& a, int w) {
+  uint32_t v = a.axis_of[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    v = w == i ? a.axis_of[i] : v;
+    asm("" : "+v"(v));
+  }
+  return v;
 }
 
 constexpr int kTileTokens = 32;            // at most
@@ -160,29 +190,32 @@ __device__ __forceinline__ void rotate_unit(float* lo, float* hi, const float* c
   }
 }
 
-// The tables' entries for pairs 8 u .. 8 u + 7 of token t, which is placed:
-// one row of them where the pairs share an axis, else each from its axis' row.
-__device__ __forceinline__ void axes_turn(const TileAppend& a, int64_t t, int u, int half, float* c, float* s) {
-  const uint32_t of = a.axis_of[u / 2] >> (16 * (u & 1)) & 0xffffu;
-  if (of == (of & 3) * 0x5555u) {
-    const int64_t at = (int64_t)a.positions[(of & 3) * (int64_t)a.num_tokens + t] * half + 8 * u;
-    load8f<Kind::F32>(a.cos_table, at, c);
-    load8f<Kind::F32>(a.sin_table, at, s);
-    return;
-  }
-  int pos[4];
+// The tables' entries for pairs 8 u .. 8 u + 7 of a token in its places: the
+// pairs of one row of them where they share an axis, else of every axis' row,
+// of which each pair keeps its own (the lanes of a token's units read whole
+// rows so; with a read for each pair 32.3 us for 4180 tokens of 32/8 heads with
+// the pairs dealt out in turn, 29.7 so, 25.4 in runs).
+__device__ __forceinline__ void axes_turn(const TileAppend& a, const Places& at, int u, int half, float* c, float* s) {
+  const uint32_t of = axes_word(a, u / 2) >> (16 * (u & 1)) & 0xffffu;
+  int64_t row = (int64_t)at.on(of & 3) * half + 8 * u;
+  load8f<Kind::F32>(a.cos_table, row, c);
+  load8f<Kind::F32>(a.sin_table, row, s);
+  if (of == (of & 3) * 0x5555u) return;
+  for (int x = 0; x < a.num_axes; ++x) {
+    float cx[8], sx[8];
+    row = (int64_t)at.on(x) * half + 8 * u;
+    load8f<Kind::F32>(a.cos_table, row, cx);
+    load8f<Kind::F32>(a.sin_table, row, sx);
 #pragma unroll
-  for (int x = 0; x < 4; ++x) pos[x] = a.positions[min(x, a.num_axes - 1) * (int64_t)a.num_tokens + t];
-#pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int x = of >> (2 * p) & 3;
-    const int64_t at = (int64_t)(x < 2 ? (x == 0 ? pos[0] : pos[1]) : (x == 2 ? pos[2] : pos[3])) * half + 8 * u + p;
-    c[p] = a.cos_table[at];
-    s[p] = a.sin_table[at];
+    for (int p = 0; p < 8; ++p) {
+      const bool mine = (of >> (2 * p) & 3) == (uint32_t)x;
+      c[p] = mine ? cx[p] : c[p];
+      s[p] = mine ? sx[p] : s[p];
+    }
   }
 }
 
-template <Kind K, int STYLE, bool AXES = false>
+template <Kind K, int STYLE>
 __device__ __forceinline__ void rotate_q_tile(const TileAppend& a, int wg) {
   const int half = a.head_size / 2, units = half / 8;
   const int sets = (a.num_heads + kTileHeadsPerThread - 1) / kTileHeadsPerThread;
@@ -191,32 +224,90 @@ __device__ __forceinline__ void rotate_q_tile(const TileAppend& a, int wg) {
   const int set = (int)((idx / units) % sets);
   const int64_t t = idx / ((int64_t)units * sets);
   if (t >= a.num_tokens) return;
+  const int pos = a.positions[t];
+  if (pos < 0 || pos >= a.max_positions) return;                // token left as it is
   float c[8], s[8], lo[kTileHeadsPerThread][8], hi[kTileHeadsPerThread][8];
-  if constexpr (AXES) {
-    if (!placed(a, t)) return;                                  // token left as it is
-    axes_turn(a, t, u, half, c, s);
-  } else {
-    const int pos = a.positions[t];
-    if (pos < 0 || pos >= a.max_positions) return;              // token left as it is
-    load8f<Kind::F32>(a.cos_table, (int64_t)pos * half + 8 * u, c);
-    load8f<Kind::F32>(a.sin_table, (int64_t)pos * half + 8 * u, s);
-  }
-  const int64_t from = AXES ? t * a.q_stride : t * a.num_heads * a.head_size;
-  const int64_t to = AXES ? t * a.q_out_stride : from;
+  load8f<Kind::F32>(a.cos_table, (int64_t)pos * half + 8 * u, c);
+  load8f<Kind::F32>(a.sin_table, (int64_t)pos * half + 8 * u, s);
   // head set + sets i: the lanes of a wavefront on consecutive heads
 #pragma unroll
   for (int i = 0; i < kTileHeadsPerThread; ++i) {
     const int h = set + i * sets;
     if (h < a.num_heads)
-      load_unit<K, STYLE>(a.q, from + h * a.head_size, u, half, lo[i], hi[i]);
+      load_unit<K, STYLE>(a.q, (t * a.num_heads + h) * a.head_size, u, half, lo[i], hi[i]);
   }
 #pragma unroll
   for (int i = 0; i < kTileHeadsPerThread; ++i) {
     const int h = set + i * sets;
     if (h >= a.num_heads) break;
     rotate_unit<STYLE>(lo[i], hi[i], c, s);
-    const int64_t base = to + h * a.head_size;
+    const int64_t base = (t * a.num_heads + h) * a.head_size;
     store_unit<K, STYLE>(a.q_out, base, u, half, lo[i], hi[i]);
+  }
+}
+
+// AXES: the q heads of one token, of more where it has few.  A thread reads the
+// tables' entries of one pair of one token, which all of the token's heads take
+// from LDS, so that pairs whose axes differ cost one read each, not one for
+// every head; the heads' first elements are on their way meanwhile.  Bound by
+// HBM: 4055 tokens of 64/8 heads into scaled FP8 pools 36.9 us, 4.3 TB/s (with
+// 4 tokens to a workgroup, of whose 8 units a thread 4 are in flight, 43.5; as
+// rotate_q_tile, the tables read by every thread, 46.0).
+inline __host__ __device__ int axes_q_tokens(int num_heads, int head_size) {
+  const int fit = kTileThreads / (head_size / 2), units = num_heads * (head_size / 16);
+  return max(1, min(fit, kTileThreads / units));
+}
+template <Kind K, int STYLE>
+__device__ __forceinline__ void rotate_q_axes(const TileAppend& a, int wg) {
+  __shared__ __attribute__((aligned(16))) float cs[kTileThreads], sn[kTileThreads];
+  __shared__ int in_tables[kTileThreads / 8];
+  const int half = a.head_size / 2, units = half / 8, tokens = axes_q_tokens(a.num_heads, a.head_size);
+  const int tid = threadIdx.x, t0 = wg * tokens;
+  const int mine = tid / half;                                  // token of the tile
+  const bool turns = mine < tokens && t0 + mine < a.num_tokens;
+  const Places at(a, turns ? t0 + mine : t0);
+  // units of the tile's tokens and heads: kAhead of a thread in flight at once
+  constexpr int kAhead = 2;
+  const unsigned per_token = (unsigned)units * a.num_heads;
+  const unsigned total = per_token * min(tokens, a.num_tokens - t0);
+  Raw8<K> lo[kAhead], hi[kAhead];
+  struct Unit { int u, t; int64_t h; };
+  auto unit_of = [&](unsigned j) {
+    const unsigned t = j / per_token, r = j - t * per_token, h = r / units;
+    return Unit{(int)(r - h * units), (int)t, (int64_t)h * a.head_size};
+  };
+  auto load = [&](unsigned j0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const Unit x = unit_of(min(j0 + i * kTileThreads, total - 1));      // past the end: the last one again
+      const int64_t from = (t0 + x.t) * a.q_stride + x.h;
+      lo[i].load(a.q, from + (STYLE == 0 ? 16 * x.u : 8 * x.u));
+      hi[i].load(a.q, from + (STYLE == 0 ? 16 * x.u + 8 : half + 8 * x.u));
+    }
+  };
+  load(tid);
+  if (turns) {
+    const int i = tid - mine * half;
+    const bool in = at.in_tables(a);
+    const int64_t row = (int64_t)(in ? at.on(axes_word(a, i / 16) >> (2 * (i % 16)) & 3) : 0) * half + i;
+    cs[tid] = a.cos_table[row];
+    sn[tid] = a.sin_table[row];
+    if (i == 0) in_tables[mine] = in;
+  }
+  __syncthreads();
+  for (unsigned j0 = tid; j0 < total; j0 += kAhead * kTileThreads) {
+    if (j0 >= kAhead * kTileThreads) load(j0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (j0 + i * kTileThreads >= total) break;
+      const Unit x = unit_of(j0 + i * kTileThreads);
+      if (!in_tables[x.t]) continue;                            // token left as it is
+      float p[8], r[8];
+      lo[i].get(p);
+      hi[i].get(r);
+      rotate_unit<STYLE>(p, r, cs + x.t * half + 8 * x.u, sn + x.t * half + 8 * x.u);
+      store_unit<K, STYLE>(a.q_out, (t0 + x.t) * a.q_out_stride + x.h, x.u, half, p, r);
+    }
   }
 }
 
@@ -225,7 +316,8 @@ __global__ __launch_bounds__(kTileThreads) void append_tiles_kernel(TileAppend a
   extern __shared__ __attribute__((aligned(16))) char tile_rows[];   // written 8 bytes at a time
   if constexpr (ROPE != kNoRope) {
     if ((int)blockIdx.x >= a.kv_wgs) {
-      rotate_q_tile<SRC, ROPE, AXES>(a, blockIdx.x - a.kv_wgs);
+      if constexpr (AXES) rotate_q_axes<SRC, ROPE>(a, blockIdx.x - a.kv_wgs);
+      else rotate_q_tile<SRC, ROPE>(a, blockIdx.x - a.kv_wgs);
       return;
     }
   }
@@ -237,11 +329,16 @@ __global__ __launch_bounds__(kTileThreads) void append_tiles_kernel(TileAppend a
 
   // lane i: token t0 + i, and the token before it
   auto slot_of = [&](int t) {
+    if constexpr (ROPE != kNoRope && AXES) {
+      // reads that wait for nothing, of the nearest token there is
+      const int near = min(max(t, 0), a.num_tokens - 1);
+      const int s = a.slots[near];
+      const Places at(a, near);
+      return t == near && s >= 0 && s / a.block_size < a.num_blocks && at.in_tables(a) ? s : -1;
+    }
     if (t < 0 || t >= a.num_tokens) return -1;
     int s = a.slots[t];
-    if constexpr (ROPE != kNoRope && AXES) {
-      s = placed(a, t) ? s : -1;
-    } else if constexpr (ROPE != kNoRope) {
+    if constexpr (ROPE != kNoRope) {
       const int p = a.positions[t];
       s = p >= 0 && p < a.max_positions ? s : -1;
     }
@@ -276,6 +373,15 @@ __global__ __launch_bounds__(kTileThreads) void append_tiles_kernel(TileAppend a
   };
   __shared__ float scale_of[SCALED ? kWave : 1];                // of the tile's rows
   if (ROPE != kNoRope && !is_v) {
+    // AXES: the tokens' places, a copy for each wavefront
+    __shared__ __attribute__((aligned(16))) Places places[AXES ? kTileThreads : 1];
+    Places* of_token = places + (AXES ? tid / kWave * kWave : 0);
+    if constexpr (ROPE != kNoRope && AXES) {
+      of_token[lane] = Places(a, min(t0 + lane, a.num_tokens - 1));
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
     if constexpr (ROPE != kNoRope) {
       const int half = a.head_size / 2, units = half / 8;
       for (int j = tid; j < (hi - lo) * units; j += kTileThreads) {
@@ -283,7 +389,7 @@ __global__ __launch_bounds__(kTileThreads) void append_tiles_kernel(TileAppend a
         if (!(mine >> i & 1)) continue;
         float c[8], s[8], x[8], y[8];
         if constexpr (AXES) {
-          axes_turn(a, t0 + i, u, half, c, s);
+          axes_turn(a, of_token[i], u, half, c, s);
         } else {
           const int64_t at = (int64_t)a.positions[t0 + i] * half + 8 * u;
           load8f<Kind::F32>(a.cos_table, at, c);
@@ -402,7 +508,13 @@ inline int tile_group(int block_size, int elem) {
 inline int64_t tile_kv_wgs(const TileAppend& a, int tile) {
   return ((int64_t)a.num_tokens + tile - 1) / tile * a.num_kv_heads * 2;
 }
-inline int64_t tile_q_wgs(const TileAppend& a) {
+template <bool AXES>
+int64_t tile_q_wgs(const TileAppend& a) {
+  if constexpr (AXES) {
+    if (a.num_heads == 0) return 0;
+    const int tokens = axes_q_tokens(a.num_heads, a.head_size);
+    return ((int64_t)a.num_tokens + tokens - 1) / tokens;
+  }
   const int64_t sets = (a.num_heads + kTileHeadsPerThread - 1) / kTileHeadsPerThread;
   return (a.num_tokens * sets * (a.head_size / 16) + kTileThreads - 1) / kTileThreads;
 }
@@ -412,11 +524,12 @@ inline int64_t tile_q_wgs(const TileAppend& a) {
 // workgroups (63 rows of 512 bytes: 32 KiB), and fewer than 2^32 threads,
 // past which a launch wraps (rows below 128 channels take more of them here
 // than in the kernels that store elements).
-inline bool tile_shape(const TileAppend& a, int src_elem, int elem, bool rope) {
+template <bool AXES = false>
+bool tile_shape(const TileAppend& a, int src_elem, int elem, bool rope) {
   auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
   if (!al(a.key) || !al(a.value) || !al(a.k_cache) || !al(a.v_cache)) return false;
   if (rope && (!al(a.cos_table) || !al(a.sin_table) || !al(a.q) || !al(a.q_out))) return false;
-  if (tile_kv_wgs(a, kTileTokens) + (rope ? tile_q_wgs(a) : 0) >= (1ll << 32) / kTileThreads) return false;
+  if (tile_kv_wgs(a, kTileTokens) + (rope ? tile_q_wgs<AXES>(a) : 0) >= (1ll << 32) / kTileThreads) return false;
   return a.block_size * elem % 16 == 0 && tile_group(a.block_size, elem) != 0 && a.head_size * elem <= 512 &&
          (int64_t)a.head_size * src_elem % 16 == 0 && a.head_size * elem % 8 == 0;
 }
@@ -435,7 +548,7 @@ int launch_tiles(TileAppend a, hipStream_t stream) {
   const int64_t full = tile_kv_wgs(a, kTileTokens);
   a.tile = full <= 64 ? 8 : full <= 256 ? 16 : kTileTokens;
   a.kv_wgs = (int)tile_kv_wgs(a, a.tile);
-  const unsigned grid = (unsigned)(a.kv_wgs + (ROPE != kNoRope ? tile_q_wgs(a) : 0));
+  const unsigned grid = (unsigned)(a.kv_wgs + (ROPE != kNoRope ? tile_q_wgs<AXES>(a) : 0));
   const size_t lds = (size_t)(a.tile + a.group - 1) * (a.head_size * E + kTileRowPad);
   hipLaunchKernelGGL((append_tiles_kernel<SRC, POOL, ROPE, AXES>), dim3(grid), dim3(kTileThreads), lds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : 5;

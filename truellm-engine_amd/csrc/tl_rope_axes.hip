@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(TileAppend a, int style,
   if (t >= a.num_tokens) return;
   const int h = (int)(row - t * per_token);
   const bool is_q = h < a.num_heads, is_v = h >= a.num_heads + a.num_kv_heads;
-  if (a.num_axes && !placed(a, t)) return;            // the token is left as it is
+  if (a.num_axes && !Places(a, t).in_tables(a)) return;   // the token is left as it is
   int blk = 0, off = 0;
   if (!is_q) {
     const int32_t slot = a.slots[t];
@@ -100,77 +100,39 @@ __global__ __launch_bounds__(256) void axes_rows_kernel(TileAppend a, int style,
 }
 
 // Steps: a wavefront per (token, kv head) with its key and its value, and
-// threads of 8 rotation pairs of a q head after them.  HBM has no byte masks:
-// storing a token's elements alone leaves partly written lines, each a
-// read-modify-write of memory later, so a lane rewrites the aligned SB bytes
-// of its channels' rows around the slot (the other slots with their own
-// bytes).  That needs them to be this token's: where another token of the
-// call writes into the same bytes, the elements are stored alone.
-// Lane l has the rotation pairs l and l + 64; its channels are theirs.
-template <int SB>
-struct RowBytes {
-  static constexpr int W = SB / 4;
-  uint32_t w[W];
-  __device__ __forceinline__ void load(const char* p) {
-    if constexpr (SB == 8) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x; w[1] = v.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        const u32x4 v = load16(p + 16 * i);
-        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(char* p) const {
-    if constexpr (SB == 8) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < W / 4; ++i)
-        *reinterpret_cast<u32x4*>(p + 16 * i) = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-    }
-  }
-  // element e of E bytes becomes v
-  template <int E>
-  __device__ __forceinline__ void put(int e, uint32_t v) {
-    const int at = e * E / 4, sh = 8 * (e * E % 4);
-    const uint32_t mask = (E == 4 ? 0xffffffffu : (1u << (8 * E % 32)) - 1u) << sh;
-#pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = i == at ? (w[i] & ~mask) | (v << sh) : w[i];
-  }
-};
-
-constexpr int kStepMaxTokens = 256;      // a wavefront looks over the call's slots
-
-template <Kind K, Kind POOL, int ROPE, int SB>
+// threads of 8 rotation pairs of a q head after them; lane l has the rotation
+// pairs l and l + 64 of the key, and the value's elements in their place.
+// Every load that hangs on nothing else is issued first, so a wavefront is two
+// round trips to memory and its stores.
+//
+// The elements of a row lie a block apart and are stored alone.  Rewriting the
+// aligned 16 to 64 bytes around each, as the 2-byte appends do, was measured
+// and is slower here, in pools that the caches hold and in pools that they do
+// not: 64 tokens, 8 kv heads, scaled FP8, blocks of 16: 3.5 us (rewritten 4.3),
+// of 64 5.7 (8.1), of 256 5.1 (10.6); bf16 3.8 (4.9), 5.4 (10.0), 4.9 (10.6).
+template <Kind K, Kind POOL, int ROPE>
 __global__ __launch_bounds__(kWave) void axes_step_kernel(TileAppend a) {
-  constexpr int E = KindInfo<POOL>::bytes, SLOTS = SB / E;
   const int lane = threadIdx.x, half = a.head_size / 2;
   if constexpr (ROPE != kNoRope) {
     if ((int)blockIdx.x >= a.kv_wgs) {
-      const int units = half / 8;
-      const int64_t idx = ((int64_t)blockIdx.x - a.kv_wgs) * kWave + lane;
+      const unsigned units = half / 8, idx = (blockIdx.x - a.kv_wgs) * kWave + lane;   // fewer than 2^32 threads
       const int u = (int)(idx % units), h = (int)(idx / units % a.num_heads);
-      const int64_t t = idx / ((int64_t)units * a.num_heads);
+      const int64_t t = idx / units / a.num_heads;
       if (t >= a.num_tokens) return;
       float c[8], s[8], lo[8], hi[8];
+      const Places at(a, t);
       load_unit<K, ROPE>(a.q, t * a.q_stride + h * a.head_size, u, half, lo, hi);
-      if (!placed(a, t)) return;                              // the token is left as it is
-      axes_turn(a, t, u, half, c, s);
+      if (!at.in_tables(a)) return;                           // the token is left as it is
+      axes_turn(a, at, u, half, c, s);
       rotate_unit<ROPE>(lo, hi, c, s);
       store_unit<K, ROPE>(a.q_out, t * a.q_out_stride + h * a.head_size, u, half, lo, hi);
       return;
     }
   }
   const int t = blockIdx.x / a.num_kv_heads, h = blockIdx.x % a.num_kv_heads;
-  // everything that hangs on nothing else goes out first
+  Places at = {};
+  if constexpr (ROPE != kNoRope) at = Places(a, t);
   const int32_t slot = a.slots[t];
-  int32_t others[kStepMaxTokens / kWave];
-#pragma unroll
-  for (int i = 0; i < kStepMaxTokens / kWave; ++i)
-    others[i] = kWave * i + lane < a.num_tokens ? a.slots[kWave * i + lane] : -1;
   float k[2][2] = {}, v[2][2] = {};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -183,85 +145,62 @@ __global__ __launch_bounds__(kWave) void axes_step_kernel(TileAppend a) {
     v[j][0] = load_scalar<K>(a.value, fv + e0);
     v[j][1] = load_scalar<K>(a.value, fv + e1);
   }
-  if (ROPE != kNoRope && !placed(a, t)) return;
+  if (ROPE != kNoRope && !at.in_tables(a)) return;
   if (slot < 0 || slot / a.block_size >= a.num_blocks) return;
   const int blk = slot / a.block_size, off = slot % a.block_size;
   const int64_t head = (int64_t)blk * a.num_kv_heads + h;
-  char* kp = a.k_cache + (head * a.head_size * a.block_size + off / SLOTS * SLOTS) * E;
-  char* vp = a.v_cache + (head * a.head_size * a.block_size + off / SLOTS * SLOTS) * E;
-  const int64_t channel = (int64_t)a.block_size * E;
-  // whether the bytes around the slot are this token's alone
-  bool other = false;
-#pragma unroll
-  for (int i = 0; i < kStepMaxTokens / kWave; ++i)
-    other |= others[i] >= 0 && others[i] / SLOTS == slot / SLOTS && kWave * i + lane != t;
-  const bool alone = __builtin_amdgcn_ballot_w64(other) == 0;
-  RowBytes<SB> kr[2][2], vr[2][2];
-  if (alone) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (lane + kWave * j >= half) break;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int64_t c = rope_channel<ROPE>(lane + kWave * j, r, half) * channel;
-        kr[j][r].load(kp + c);
-        vr[j][r].load(vp + c);
-      }
-    }
-  }
   uint32_t kt = 0, vt = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = lane + kWave * j;
     if (i >= half) break;
     if constexpr (ROPE != kNoRope) {
-      const int axis = a.axis_of[i / 16] >> (2 * (i % 16)) & 3;
-      const int64_t at = (int64_t)a.positions[axis * (int64_t)a.num_tokens + t] * half + i;
-      const float c = a.cos_table[at], s = a.sin_table[at], x0 = k[j][0], x1 = k[j][1];
+      const int64_t row = (int64_t)at.on(axes_word(a, i / 16) >> (2 * (i % 16)) & 3) * half + i;
+      const float c = a.cos_table[row], s = a.sin_table[row], x0 = k[j][0], x1 = k[j][1];
       k[j][0] = fp32_result(__builtin_fmaf(x0, c, -(x1 * s)));
       k[j][1] = fp32_result(__builtin_fmaf(x0, s, x1 * c));
     }
     kt = max(kt, max(abs_bits(k[j][0]), abs_bits(k[j][1])));
     vt = max(vt, max(abs_bits(v[j][0]), abs_bits(v[j][1])));
   }
-  Fp8Scale ks = {}, vs = {};
+  const int64_t to = head * a.head_size * a.block_size + off;
   if constexpr (POOL == Kind::FP8) {
-    ks = fp8_scale_of(lanes_umax<kWave>(kt));
-    vs = fp8_scale_of(lanes_umax<kWave>(vt));
+    const Fp8Scale ks = fp8_scale_of(lanes_umax<kWave>(kt)), vs = fp8_scale_of(lanes_umax<kWave>(vt));
     if (lane == 0) {
       a.k_scales[head * a.block_size + off] = ks.scale;
       a.v_scales[head * a.block_size + off] = vs.scale;
     }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        k[j][r] *= ks.inv;
+        v[j][r] *= vs.inv;
+      }
   }
-  auto bits = [&](float x, const Fp8Scale& sc) -> uint32_t {
-    if constexpr (POOL == Kind::FP8) return f32_to_fp8(x * sc.inv);
-    else return scalar_bits<POOL>(x);
-  };
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     if (lane + kWave * j >= half) break;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t c = rope_channel<ROPE>(lane + kWave * j, r, half) * channel;
-      const uint32_t kb = bits(k[j][r], ks), vb = bits(v[j][r], vs);
-      if (alone) {
-        kr[j][r].template put<E>(off % SLOTS, kb);
-        vr[j][r].template put<E>(off % SLOTS, vb);
-        kr[j][r].store(kp + c);
-        vr[j][r].store(vp + c);
-      } else if constexpr (E == 1) {
-        *(uint8_t*)(kp + c + off % SLOTS) = (uint8_t)kb;
-        *(uint8_t*)(vp + c + off % SLOTS) = (uint8_t)vb;
-      } else if constexpr (E == 2) {
-        *(uint16_t*)(kp + c + off % SLOTS * E) = (uint16_t)kb;
-        *(uint16_t*)(vp + c + off % SLOTS * E) = (uint16_t)vb;
+      const int64_t e = to + (int64_t)rope_channel<ROPE>(lane + kWave * j, r, half) * a.block_size;
+      if constexpr (POOL == Kind::FP8) {
+        ((uint8_t*)a.k_cache)[e] = f32_to_fp8(k[j][r]);
+        ((uint8_t*)a.v_cache)[e] = f32_to_fp8(v[j][r]);
       } else {
-        *(uint32_t*)(kp + c + off % SLOTS * E) = kb;
-        *(uint32_t*)(vp + c + off % SLOTS * E) = vb;
+        store_scalar<POOL>(a.k_cache, e, k[j][r]);
+        store_scalar<POOL>(a.v_cache, e, v[j][r]);
       }
     }
   }
 }
+
+// Rows of keys up to which a call is taken for a step.  us as a step and in
+// tiles, one run of consecutive tokens and tokens that each lie in a block of
+// their own, blocks of 64, bf16: 8/1 heads, 600 tokens 4.4 and 6.1, 5.3 and
+// 6.7; 16/2, 600 5.6 and 5.5, 7.4 and 8.6; past the line 32/8, 300 6.9 and 5.9,
+// 11.4 and 12.6, 600 11.0 and 7.3, 33.5 and 32.8; 32/32, 300 15.7 and 8.1.
+constexpr int64_t kStepMaxRows = 2048;
 
 template <Kind K, Kind POOL, int ROPE>
 int launch_style(const TileAppend& a, int style, hipStream_t stream) {
@@ -271,28 +210,19 @@ int launch_style(const TileAppend& a, int style, hipStream_t stream) {
   const bool rows16 = ROPE == kNoRope || a.num_heads == 0 ||
                       (al(a.q) && al(a.q_out) && whole(a.q_stride) && whole(a.q_out_stride));
   const bool tables16 = ROPE == kNoRope || (al(a.cos_table) && al(a.sin_table));
-  const bool pools16 = al(a.k_cache) && al(a.v_cache);
-  if (a.num_tokens <= kStepMaxTokens && rows16 && tables16 && pools16) {
-    // the bytes of a channel's row around a slot: up to 64
-    const int row = a.block_size * E;
-    const int sb = row % 64 == 0 ? 64 : row == 32 || row == 16 || row == 8 ? row : 0;
+  if ((int64_t)a.num_tokens * a.num_kv_heads > kStepMaxRows && rows16 && whole(a.key_stride) && whole(a.value_stride) &&
+      tile_shape<true>(a, S, E, ROPE != kNoRope))
+    return launch_tiles<K, POOL, ROPE, true>(a, stream);
+  if (rows16 && tables16) {
     TileAppend s = a;
     s.kv_wgs = a.num_tokens * a.num_kv_heads;
     const int64_t q = ROPE == kNoRope ? 0 : (int64_t)a.num_tokens * a.num_heads * (a.head_size / 16);
     const int64_t wgs = (int64_t)a.num_tokens * a.num_kv_heads + (q + kWave - 1) / kWave;
-    if (sb && wgs < (1ll << 32) / kWave) {
-      const dim3 grid((unsigned)wgs);
-      auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kWave), 0, stream, s); };
-      if (sb == 64) go(axes_step_kernel<K, POOL, ROPE, 64>);
-      else if (sb == 32) go(axes_step_kernel<K, POOL, ROPE, 32>);
-      else if (sb == 16) go(axes_step_kernel<K, POOL, ROPE, 16>);
-      else go(axes_step_kernel<K, POOL, ROPE, 8>);
+    if (wgs < (1ll << 32) / kWave) {
+      hipLaunchKernelGGL((axes_step_kernel<K, POOL, ROPE>), dim3((unsigned)wgs), dim3(kWave), 0, stream, s);
       return hipGetLastError() == hipSuccess ? 0 : 5;
     }
   }
-  if (a.num_tokens > kStepMaxTokens && rows16 && whole(a.key_stride) && whole(a.value_stride) &&
-      tile_shape(a, S, E, ROPE != kNoRope))
-    return launch_tiles<K, POOL, ROPE, true>(a, stream);
   const int64_t rows = (int64_t)a.num_tokens * (a.num_heads + 2 * a.num_kv_heads), wgs = (rows + 3) / 4;
   constexpr int64_t kWgs = 1 << 23;                   // of a launch: fewer than 2^32 threads
   for (int64_t w = 0; w < wgs; w += kWgs)

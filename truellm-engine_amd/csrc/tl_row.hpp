@@ -1,5 +1,5 @@
-// tl_row.hpp -- what the kernels that work on rows of activations share:
-// eight elements between storage and fp32, and a row's sum over a workgroup.
+// tl_row.hpp -- what the kernels that work on rows of activations or heads
+// share: eight elements between storage and fp32, a row's sum over a workgroup.
 #pragma once
 
 #include "tl_device.hpp"
@@ -52,6 +52,36 @@ template <Kind K> __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
     w[k] = (uint32_t)lo | ((uint32_t)hi << 16);
   }
   return u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// Eight elements as loaded.
+template <Kind K> struct Raw8 {
+  u32x4 w[K == Kind::F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    const char* at = (const char*)p + i * KindInfo<K>::bytes;
+    w[0] = load16(at);
+    if constexpr (K == Kind::F32) w[1] = load16(at + 16);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (K == Kind::F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(float, word(w[j / 4], j % 4));
+    } else {
+      unpack8<K>(w[0], f);
+    }
+  }
+};
+template <Kind K>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&f)[8]) {
+  char* at = (char*)p + i * KindInfo<K>::bytes;
+  if constexpr (K == Kind::F32) {
+    u32x4 w[2];
+    __builtin_memcpy(w, f, 32);
+    reinterpret_cast<u32x4*>(at)[0] = w[0];
+    reinterpret_cast<u32x4*>(at)[1] = w[1];
+  } else {
+    *reinterpret_cast<u32x4*>(at) = pack8<K>(f);
+  }
 }
 
 }  // namespace tl
