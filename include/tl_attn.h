@@ -297,10 +297,9 @@ int tl_rope_reshape_and_cache(const void* q, void* q_out, const void* key, const
  * the scales as they move pools (block_bytes n_kv * block_size * 4).
  * tl_reshape_and_cache_fp8 with such scales: key / value [T, n_kv,
  * head_size] of src_dtype F16 or BF16, head_size 128, any block_size; slots
- * as there (< 0 or past the pool: nothing written), none twice in a call.
- * Calls of few tokens rewrite the bytes around a token's slot (up to its
- * block's rows of a kv head, the other slots with their own bytes), so a
- * block that the call writes to has no other writer during it. */
+ * as there (< 0 or past the pool: nothing written), none twice in a call (a
+ * row's codes and its scale could be of different tokens).  No slot but the
+ * call's own is written. */
 int tl_reshape_and_cache_fp8_scaled(const void* key, const void* value, int32_t src_dtype, uint8_t* k_cache,
                                     uint8_t* v_cache, float* k_scales, float* v_scales,
                                     const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
@@ -338,8 +337,7 @@ typedef struct tl_rope_axes_desc {
  * the next of q, q_out, key and value (0: the heads' own size), so that
  * slices of one projection's output can be passed; a head's elements and a
  * token's heads are contiguous.  Slots as for
- * tl_reshape_and_cache_fp8_scaled; calls of few tokens rewrite bytes around
- * their slots as that call does, into pools of either type. */
+ * tl_reshape_and_cache_fp8_scaled, into pools of either type. */
 int tl_rope_axes_reshape_and_cache(const tl_rope_axes_desc* desc, const void* q, void* q_out, const void* key,
                                    const void* value, void* k_cache, void* v_cache, float* k_scales,
                                    float* v_scales, const int32_t* slot_mapping, const int32_t* positions,

@@ -10,9 +10,9 @@
 // tensors' own type takes the result rounded once; an FP8 pool takes
 //   scale = max|row| / 448,  code = e4m3(row / scale)
 // of each row (one token of one kv head; the key as rotated, in fp32).
-// Prompts go through the tiles of tl_append_tiles.hpp, steps (few tokens, as a
-// rule each in a block of its own) through axes_step_kernel; what neither
-// takes (odd strides, alignments and block sizes) through axes_rows_kernel.
+// Prompts go through the tiles of tl_append_tiles.hpp, steps (few rows) and
+// blocks that hold no whole 16-byte chunks through axes_step_kernel; rows or
+// tables that are not 16-byte aligned through axes_rows_kernel.
 #include "tl_append_tiles.hpp"
 #include "tl_device.hpp"
 #include "tl_fp8.hpp"
