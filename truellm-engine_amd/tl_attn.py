@@ -290,9 +290,15 @@ def _on_gpu(*tensors):
 
 
 def _stream(stream=None):
+    """The stream's handle; without one, that of the current device's current stream (read as torch's own launchers
+    read it: the stream object costs as much as a launch)."""
+    if stream is not None:
+        return stream.cuda_stream
     torch = _torch()
-    s = torch.cuda.current_stream() if stream is None else stream
-    return ctypes.c_void_p(s.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_stream().cuda_stream
+    return raw(torch.cuda.current_device())
 
 
 # ---------------------------------------------------------------------------
