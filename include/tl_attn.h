@@ -116,7 +116,8 @@ int tl_paged_attention_decode(const tl_decode_desc* desc, void* out, const void*
  * block_size] beside the pools,
  *   s_t = scale * k_scales_t (q . kcode_t),
  *   out = sum_t softmax(s)_t v_scales_t vcode_t.
- * desc->kv_dtype FP8_E4M3, head_size 128; k_scale / v_scale are ignored.  The
+ * Scales are >= 0 (or NaN), values of any size.  desc->kv_dtype FP8_E4M3,
+ * head_size 128; k_scale / v_scale are ignored.  The
  * plan and the workspace (tl_paged_attention_workspace_bytes) are those of
  * the call without scales.  Scales past a sequence's length or in blocks that
  * it does not name may hold anything.  A value of scale NaN makes its
@@ -329,7 +330,8 @@ typedef struct tl_rope_axes_desc {
   int32_t max_positions;       /* rows of the tables */
 } tl_rope_axes_desc;
 
-/* q [T, num_heads, d] -> q_out (may be q), key / value [T, n_kv, d] into the
+/* q [T, num_heads, d] -> q_out (may be q, of one stride; overlaps no other
+ * tensor), key / value [T, n_kv, d] into the
  * pools; k_scales / v_scales as above for FP8 pools (of the rotated key,
  * which is not rounded to dtype first), NULL otherwise.  positions int32
  * [num_axes, T]; a token with a position outside [0, max_positions) on some

@@ -275,3 +275,33 @@ def test_scaled_prefill_binding_refuses_wrong_tensors():
         a = {**good, **kw}
         with pytest.raises(tla.TLError):
             tla.chunked_prefill_scaled(desc, a["out"], a["q"], a["cu"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["sl"], 4)
+
+
+def test_appends_refuse_rows_and_strides_past_int32():
+    d = _axes_desc(num_heads=2**24)
+    assert _axes(d) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(_axes_desc(num_kv_heads=2**24)) == tla.ERR_INVALID_ARGUMENT
+    assert L.tl_reshape_and_cache_fp8_scaled(FAKE, FAKE, tla.F16, FAKE, FAKE, FAKE, FAKE, FAKE, 4, 2**24, 128, 16, 64,
+                                             None) == tla.ERR_INVALID_ARGUMENT
+    far = torch.empty(2**31 + 256, dtype=torch.bfloat16, device="meta").as_strided((2, 2, 128), (2**31, 128, 1))
+    with pytest.raises(tla.TLError, match="tokens less than 2\\^31 apart"):
+        tla._token_stride(far, 2, 2, 128, tla.BF16, "key")
+    assert tla._token_stride(far[:, :, :].as_strided((2, 2, 128), (2**31 - 1, 128, 1)), 2, 2, 128, tla.BF16, "key") \
+        == 2**31 - 1
+
+
+def test_rope_axes_refuses_two_strides_in_place():
+    # one token has none; the others would be read where an earlier one was written
+    d = _axes_desc()
+    assert _axes(d, strides=(2048, 1024, 0, 0)) == tla.ERR_INVALID_ARGUMENT
+    assert _axes(d, strides=(0, 2048, 0, 0)) == tla.ERR_INVALID_ARGUMENT
+
+
+def test_scaled_decode_refuses_a_strided_workspace():
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    q, pool, scales = torch.zeros(3, 8, 128, dtype=bf), torch.zeros(6, 2, 128, 16, dtype=u8), torch.zeros(6, 2, 16)
+    tables, lens = torch.zeros(3, 5, dtype=i32), torch.zeros(3, dtype=i32)
+    desc = tla.make_decode_desc(q, pool, tables, 2, 0.1)
+    with pytest.raises(tla.TLError, match="workspace"):
+        tla.paged_attention_decode_scaled(desc, q.clone(), q, pool, pool, scales, scales, tables, lens, 80,
+                                          torch.zeros(1, dtype=u8).expand(1 << 20))

@@ -533,9 +533,11 @@ int tl_rope_reshape_and_cache(const void* q, void* q_out, const void* key, const
 }
 
 // Slots are int32: a pool past 2^31 of them has blocks that none can name.
-static int check_slots(int32_t num_blocks, int32_t block_size) {
+// So are the elements of a token's heads.
+static int check_slots(int32_t num_blocks, int32_t block_size, int64_t row) {
   if ((int64_t)num_blocks * block_size > ((int64_t)1 << 31))
     return fail(TL_ERR_INVALID_ARGUMENT, "num_blocks=%d x block_size=%d slots exceed int32", num_blocks, block_size);
+  if (row > INT32_MAX) return fail(TL_ERR_INVALID_ARGUMENT, "%lld elements of a token exceed int32", (long long)row);
   return TL_OK;
 }
 
@@ -548,7 +550,7 @@ int tl_reshape_and_cache_fp8_scaled(const void* key, const void* value, int32_t 
                 num_tokens, num_kv_heads, head_size, block_size, num_blocks);
   if (src_dtype != TL_DTYPE_F16 && src_dtype != TL_DTYPE_BF16)
     return fail(TL_ERR_NOT_IMPLEMENTED, "src_dtype=%d (F16 or BF16 sources)", src_dtype);
-  int rc = check_slots(num_blocks, block_size);
+  int rc = check_slots(num_blocks, block_size, (int64_t)num_kv_heads * head_size);
   if (rc) return rc;
   if (num_tokens == 0) return ok();
   rc = check_scales(k_scales, v_scales, head_size);
@@ -606,7 +608,7 @@ int tl_rope_axes_reshape_and_cache(const tl_rope_axes_desc* d, const void* q, vo
       (key_stride && key_stride < kv_row) || (value_stride && value_stride < kv_row))
     return fail(TL_ERR_INVALID_ARGUMENT, "strides q=%d q_out=%d key=%d value=%d below a token's heads", q_stride,
                 q_out_stride, key_stride, value_stride);
-  int rc = check_slots(d->num_blocks, d->block_size);
+  int rc = check_slots(d->num_blocks, d->block_size, q_row + 2 * kv_row);
   if (rc) return rc;
   if (num_tokens == 0) return ok();
   if (fp8) {
@@ -622,6 +624,9 @@ int tl_rope_axes_reshape_and_cache(const tl_rope_axes_desc* d, const void* q, vo
   if (((uintptr_t)key | (uintptr_t)value | (uintptr_t)q | (uintptr_t)q_out) & el ||
       (!fp8 && ((uintptr_t)k_cache | (uintptr_t)v_cache) & el))
     return fail(TL_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+  if (d->num_heads > 0 && num_tokens > 1 && q == q_out &&
+      (q_stride ? q_stride : q_row) != (q_out_stride ? q_out_stride : q_row))
+    return fail(TL_ERR_INVALID_ARGUMENT, "q in place with strides q=%d q_out=%d", q_stride, q_out_stride);
   tl::AxesAppend a;
   memset(&a, 0, sizeof a);
   a.q = q; a.q_out = q_out; a.key = key; a.value = value; a.k_cache = k_cache; a.v_cache = v_cache;

@@ -242,9 +242,10 @@ struct ValueUnit {
     top = __builtin_bit_cast(float, lanes_umax_32(lanes_umax<16>(__builtin_bit_cast(uint32_t, v))));
     return __builtin_amdgcn_ballot_w64(top > 64.f * unit) != 0;
   }
-  // the factor of what was summed so far
+  // the factor of what was summed so far (2^-90 at least: the weights then
+  // reach 2^98, and a sum of them over any length stays finite)
   __device__ __forceinline__ float raise(float top) {
-    const int x = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
+    const int x = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -90), 100);
     const float f = __builtin_amdgcn_exp2f(e - (float)x);
     e = (float)x;
     unit = __builtin_bit_cast(float, (uint32_t)(x + 127) << 23);

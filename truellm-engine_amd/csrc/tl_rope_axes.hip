@@ -215,10 +215,10 @@ int launch_style(const TileAppend& a, int style, hipStream_t stream) {
     return launch_tiles<K, POOL, ROPE, true>(a, stream);
   if (rows16 && tables16) {
     TileAppend s = a;
-    s.kv_wgs = a.num_tokens * a.num_kv_heads;
     const int64_t q = ROPE == kNoRope ? 0 : (int64_t)a.num_tokens * a.num_heads * (a.head_size / 16);
     const int64_t wgs = (int64_t)a.num_tokens * a.num_kv_heads + (q + kWave - 1) / kWave;
     if (wgs < (1ll << 32) / kWave) {
+      s.kv_wgs = a.num_tokens * a.num_kv_heads;
       hipLaunchKernelGGL((axes_step_kernel<K, POOL, ROPE>), dim3((unsigned)wgs), dim3(kWave), 0, stream, s);
       return hipGetLastError() == hipSuccess ? 0 : 5;
     }

@@ -497,9 +497,9 @@ def _token_stride(t, T, heads, head_size, dtype, what):
     """Elements from a token of t [T, heads, head_size] to the next; its heads lie together."""
     st = t.stride()
     if (t.shape != (T, heads, head_size) or dtype_code(t) != dtype or st[2] != 1
-            or (heads > 1 and st[1] != head_size) or (T > 1 and st[0] < heads * head_size)):
+            or (heads > 1 and st[1] != head_size) or (T > 1 and not heads * head_size <= st[0] < 2**31)):
         raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} strides {st}: "
-                      f"{(T, heads, head_size)} with the heads of a token together")
+                      f"{(T, heads, head_size)} with the heads of a token together, tokens less than 2^31 apart")
     return st[0] if T > 1 else 0
 
 
@@ -646,6 +646,8 @@ def paged_attention_decode_scaled(desc: DecodeDesc, out, q, k_cache, v_cache, k_
         if t.shape != (S, desc.num_heads, desc.head_size) or dtype_code(t) != desc.q_dtype or not t.is_contiguous():
             raise TLError(ERR_INVALID_ARGUMENT, f"q / out {tuple(t.shape)} {t.dtype}: contiguous "
                           f"{(S, desc.num_heads, desc.head_size)} of the descriptor's type")
+    if workspace is not None and not workspace.is_contiguous():
+        raise TLError(ERR_INVALID_ARGUMENT, f"workspace strides {workspace.stride()}: contiguous")
     _on_gpu(q, out, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, workspace)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     check(lib.tl_paged_attention_decode_scaled(
