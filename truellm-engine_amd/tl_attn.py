@@ -262,13 +262,26 @@ def _torch():
     return torch
 
 
-_CODE_OF = {}             # torch dtype -> tl_dtype
+I32 = -1                  # int32, which is not a tl_dtype
+
+
+class _Dtypes(dict):
+    """tl_dtype -> torch dtype (None: no such), filled on first use."""
+
+    def __missing__(self, code):
+        torch = _torch()
+        self.update({F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16, FP8_E4M3: torch.uint8,
+                     I32: torch.int32})
+        return self.get(code)
+
+
+_DTYPE_OF = _Dtypes()
+_CODE_OF = {}             # and back
 
 
 def dtype_code(t) -> int:
     if not _CODE_OF:
-        torch = _torch()
-        _CODE_OF.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.uint8: FP8_E4M3})
+        _CODE_OF.update({_DTYPE_OF[code]: code for code in (F32, F16, BF16, FP8_E4M3)})
     code = _CODE_OF.get(t.dtype)
     if code is None:
         raise TLError(ERR_INVALID_ARGUMENT, f"unsupported tensor dtype {t.dtype}")
@@ -280,13 +293,18 @@ def _ptr(t):
 
 
 def _on_gpu(*tensors):
-    """Refuses tensors (None aside) that are not on the current device, whose streams and kernels would not reach
-    them."""
-    first = tensors[0]
-    here = _torch().cuda.current_device() if first.is_cuda else -2
+    """The tensors' pointers (None: null); refuses one that is not on the current device, whose streams and kernels
+    would not reach it."""
+    here = _torch().cuda.current_device() if tensors[0].is_cuda else -2
+    at = []
     for t in tensors:
-        if t is not None and t.get_device() != here:
+        if t is None:
+            at.append(None)
+        elif t.get_device() == here:
+            at.append(t.data_ptr())
+        else:
             raise TLError(ERR_INVALID_ARGUMENT, f"a tensor on {t.device}, not on the current GPU")
+    return at
 
 
 def _stream(stream=None):
@@ -393,37 +411,32 @@ def fused_add_rms_norm(out, residual, x, weight, eps, stream=None):
                                     dtype_code(x), _stream(stream)))
 
 
-def _norm_fp8_sizes(out, scales, x, weight, group_size, residual=None):
-    """(T, H, dtype) of an FP8 norm's tensors, whose sizes the library cannot see."""
+def _norm_fp8(fn, out, scales, residual, x, weight, eps, group_size, stream):
+    """An FP8 norm's call (residual: () without one); the library cannot see the tensors' sizes."""
     shape, dtype = x.shape, x.dtype
     T, H = shape
     want = (T, H // group_size) if group_size > 0 else (T,)
     if not (out.shape == shape and out.element_size() == 1 and scales.shape == want and weight.shape == (H,)
-            and weight.dtype == dtype and dtype_code(scales) == F32 and x.is_contiguous() and out.is_contiguous()
+            and weight.dtype == dtype and scales.dtype is _DTYPE_OF[F32] and x.is_contiguous() and out.is_contiguous()
             and scales.is_contiguous() and weight.is_contiguous()):
         raise TLError(ERR_INVALID_ARGUMENT, f"x {tuple(shape)} {dtype}: out {tuple(out.shape)} {out.dtype}, "
                       f"scales {tuple(scales.shape)} {scales.dtype} (fp32 {want}), weight {tuple(weight.shape)} "
                       f"{weight.dtype}, all contiguous")
-    if residual is not None and not (residual.shape == shape and residual.dtype == dtype
-                                     and residual.is_contiguous()):
-        raise TLError(ERR_INVALID_ARGUMENT, f"residual {tuple(residual.shape)} {residual.dtype}")
-    _on_gpu(x, out, scales, weight, residual)
-    return T, H, dtype_code(x)
+    for r in residual:
+        if r is None or not (r.shape == shape and r.dtype == dtype and r.is_contiguous()):
+            raise TLError(ERR_INVALID_ARGUMENT, f"residual {r if r is None else (tuple(r.shape), r.dtype)}")
+    check(fn(*_on_gpu(out, scales, *residual, x, weight), T, H, group_size, eps, dtype_code(x), _stream(stream)))
 
 
 def rms_norm_fp8(out, scales, x, weight, eps, group_size=0, stream=None):
     """RMSNorm of x [T, H] as E4M3 codes out (uint8 [T, H]) under fp32 scales: [T] (group_size 0) or
     [T, H / group_size]; value = code * scale."""
-    T, H, code = _norm_fp8_sizes(out, scales, x, weight, group_size)
-    check(lib.tl_rms_norm_fp8(_ptr(out), _ptr(scales), _ptr(x), _ptr(weight), T, H, group_size, eps, code,
-                              _stream(stream)))
+    _norm_fp8(lib.tl_rms_norm_fp8, out, scales, (), x, weight, eps, group_size, stream)
 
 
 def fused_add_rms_norm_fp8(out, scales, residual, x, weight, eps, group_size=0, stream=None):
     """rms_norm_fp8 of residual + x, which replaces residual (in its dtype)."""
-    T, H, code = _norm_fp8_sizes(out, scales, x, weight, group_size, residual)
-    check(lib.tl_fused_add_rms_norm_fp8(_ptr(out), _ptr(scales), _ptr(residual), _ptr(x), _ptr(weight), T, H,
-                                        group_size, eps, code, _stream(stream)))
+    _norm_fp8(lib.tl_fused_add_rms_norm_fp8, out, scales, (residual,), x, weight, eps, group_size, stream)
 
 
 def layer_norm(out, x, weight, bias, eps, stream=None):
@@ -494,32 +507,36 @@ def make_rope_axes_desc(q, key, k_cache, axis_pairs, max_positions, *, style=ROP
 
 
 def _token_stride(t, T, heads, head_size, dtype, what):
-    """Elements from a token of t [T, heads, head_size] to the next; its heads lie together."""
+    """Elements from a token of t [T, heads, head_size] to the next (0: contiguous); its heads lie together."""
+    shape = (T, heads, head_size)
+    typed = t.shape == shape and t.dtype is _DTYPE_OF[dtype]
+    if typed and t.is_contiguous():
+        return 0
     st = t.stride()
-    if (t.shape != (T, heads, head_size) or dtype_code(t) != dtype or st[2] != 1
-            or (heads > 1 and st[1] != head_size) or (T > 1 and not heads * head_size <= st[0] < 2**31)):
+    if not typed or st[2] != 1 or (heads > 1 and st[1] != head_size) \
+            or (T > 1 and not heads * head_size <= st[0] < 2**31):
         raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} strides {st}: "
-                      f"{(T, heads, head_size)} with the heads of a token together, tokens less than 2^31 apart")
+                      f"{shape} with the heads of a token together, tokens less than 2^31 apart")
     return st[0] if T > 1 else 0
+
+
+def _check(t, shape, dtype, what):
+    """A contiguous tensor of this shape and tl_dtype (or I32)."""
+    if t.shape != shape or t.dtype is not _DTYPE_OF[dtype] or not t.is_contiguous():
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype}: contiguous {tuple(shape)} of "
+                      f"{_DTYPE_OF[dtype]}")
 
 
 def _check_pools(k_cache, v_cache, k_scales, v_scales, kv_dtype, num_blocks, heads, head_size, block_size):
     """Pools [N, n_kv, D, bs] of one type, and their scales (None: none) fp32 [N, n_kv, bs]."""
     shape = (num_blocks, heads, head_size, block_size)
-    if not (k_cache.shape == shape and v_cache.shape == shape and dtype_code(k_cache) == kv_dtype
-            and v_cache.dtype == k_cache.dtype and k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise TLError(ERR_INVALID_ARGUMENT, f"pools {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} "
-                      f"{v_cache.dtype}: contiguous {shape} of tl_dtype {kv_dtype}")
-    for s in (k_scales, v_scales):
-        if s is not None and not (s.shape == (num_blocks, heads, block_size) and dtype_code(s) == F32
-                                  and s.is_contiguous()):
-            raise TLError(ERR_INVALID_ARGUMENT, f"scales {tuple(s.shape)} {s.dtype}: contiguous fp32 "
-                          f"{(num_blocks, heads, block_size)}")
-
-
-def _check_ints(t, shape, what):
-    if t.shape != shape or t.dtype != _torch().int32 or not t.is_contiguous():
-        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype}: contiguous int32 {shape}")
+    _check(k_cache, shape, kv_dtype, "k_cache")
+    _check(v_cache, shape, kv_dtype, "v_cache")
+    shape = (num_blocks, heads, block_size)
+    if k_scales is not None:
+        _check(k_scales, shape, F32, "k_scales")
+    if v_scales is not None:
+        _check(v_scales, shape, F32, "v_scales")
 
 
 def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_cache, slot_mapping, positions, cos_table,
@@ -531,36 +548,34 @@ def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_ca
     q_out = q if q_out is None else q_out
     sq = so = 0
     if H:
-        sq, so = _token_stride(q, T, H, D, dtype, "q"), _token_stride(q_out, T, H, D, dtype, "q_out")
+        sq = _token_stride(q, T, H, D, dtype, "q")
+        so = sq if q_out is q else _token_stride(q_out, T, H, D, dtype, "q_out")
+    else:
+        q = q_out = None
     sk, sv = _token_stride(key, T, n_kv, D, dtype, "key"), _token_stride(value, T, n_kv, D, dtype, "value")
     _check_pools(k_cache, v_cache, k_scales, v_scales, desc.kv_dtype, desc.num_blocks, n_kv, D, desc.block_size)
-    _check_ints(slot_mapping, (T,), "slot_mapping")
-    _check_ints(positions, (desc.num_axes, T), "positions")
+    _check(slot_mapping, (T,), I32, "slot_mapping")
+    _check(positions, (desc.num_axes, T), I32, "positions")
     table = (desc.max_positions, D // 2)
-    for t in (cos_table, sin_table):
-        if t.shape != table or dtype_code(t) != F32 or not t.is_contiguous():
-            raise TLError(ERR_INVALID_ARGUMENT, f"table {tuple(t.shape)} {t.dtype}: contiguous fp32 {table}")
-    _on_gpu(key, value, q if H else None, q_out if H else None, k_cache, v_cache, k_scales, v_scales, slot_mapping,
-            positions, cos_table, sin_table)
-    check(lib.tl_rope_axes_reshape_and_cache(
-        ctypes.byref(desc), _ptr(q), _ptr(q_out), _ptr(key), _ptr(value), _ptr(k_cache), _ptr(v_cache),
-        _ptr(k_scales), _ptr(v_scales), _ptr(slot_mapping), _ptr(positions), _ptr(cos_table), _ptr(sin_table), T,
-        sq, so, sk, sv, _stream(stream)))
+    _check(cos_table, table, F32, "cos_table")
+    _check(sin_table, table, F32, "sin_table")
+    key_at, *at = _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, positions, cos_table, sin_table,
+                          q, q_out)
+    check(lib.tl_rope_axes_reshape_and_cache(ctypes.byref(desc), at[9], at[10], key_at, *at[:9], T, sq, so, sk, sv,
+                                             _stream(stream)))
 
 
 def reshape_and_cache_fp8_scaled(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, stream=None):
     """reshape_and_cache_fp8 with a scale for each token and head, found here: k_scales / v_scales fp32
     [N, n_kv, bs]."""
     T, n_kv, D = key.shape
-    if not (key.is_contiguous() and value.is_contiguous() and value.shape == key.shape and value.dtype == key.dtype):
-        raise TLError(ERR_INVALID_ARGUMENT, f"key {tuple(key.shape)} {key.dtype}, value {tuple(value.shape)} "
-                      f"{value.dtype}: contiguous, of one type")
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, k_cache.shape[0], n_kv, D, k_cache.shape[3])
-    _check_ints(slot_mapping, (T,), "slot_mapping")
-    _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
-    check(lib.tl_reshape_and_cache_fp8_scaled(
-        _ptr(key), _ptr(value), dtype_code(key), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
-        _ptr(slot_mapping), T, n_kv, D, k_cache.shape[3], k_cache.shape[0], _stream(stream)))
+    BS, N, code = k_cache.shape[3], k_cache.shape[0], dtype_code(key)
+    _check(key, key.shape, code, "key")
+    _check(value, key.shape, code, "value")
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, N, n_kv, D, BS)
+    _check(slot_mapping, (T,), I32, "slot_mapping")
+    key_at, value_at, *at = _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
+    check(lib.tl_reshape_and_cache_fp8_scaled(key_at, value_at, code, *at, T, n_kv, D, BS, N, _stream(stream)))
 
 
 def _block_bytes(pool):
@@ -637,22 +652,20 @@ def paged_attention_decode(desc: DecodeDesc, out, q, k_cache, v_cache, block_tab
 def paged_attention_decode_scaled(desc: DecodeDesc, out, q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
                                   max_context_len, workspace=None, stream=None):
     """paged_attention_decode over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
-    S = desc.num_seqs
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, desc.num_kv_heads, desc.head_size,
-                 desc.block_size)
-    _check_ints(block_tables, (S, desc.max_blocks_per_seq), "block_tables")
-    _check_ints(seq_lens, (S,), "seq_lens")
-    for t in (q, out):
-        if t.shape != (S, desc.num_heads, desc.head_size) or dtype_code(t) != desc.q_dtype or not t.is_contiguous():
-            raise TLError(ERR_INVALID_ARGUMENT, f"q / out {tuple(t.shape)} {t.dtype}: contiguous "
-                          f"{(S, desc.num_heads, desc.head_size)} of the descriptor's type")
-    if workspace is not None and not workspace.is_contiguous():
-        raise TLError(ERR_INVALID_ARGUMENT, f"workspace strides {workspace.stride()}: contiguous")
-    _on_gpu(q, out, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, workspace)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    check(lib.tl_paged_attention_decode_scaled(
-        ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
-        _ptr(block_tables), _ptr(seq_lens), max_context_len, _ptr(workspace), ws_bytes, _stream(stream)))
+    S, n_kv, D = desc.num_seqs, desc.num_kv_heads, desc.head_size
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size)
+    _check(block_tables, (S, desc.max_blocks_per_seq), I32, "block_tables")
+    _check(seq_lens, (S,), I32, "seq_lens")
+    rows = (S, desc.num_heads, D)
+    _check(q, rows, desc.q_dtype, "q")
+    _check(out, rows, desc.q_dtype, "out")
+    ws_bytes = 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise TLError(ERR_INVALID_ARGUMENT, f"workspace strides {workspace.stride()}: contiguous")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    *at, ws = _on_gpu(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, workspace)
+    check(lib.tl_paged_attention_decode_scaled(ctypes.byref(desc), *at, max_context_len, ws, ws_bytes, _stream(stream)))
 
 
 NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -844,21 +857,16 @@ def chunked_prefill(desc, out, q, cu_q_lens, k_cache, v_cache, block_tables, seq
 def chunked_prefill_scaled(desc, out, q, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
                            max_q_len, stream=None):
     """chunked_prefill over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
-    S = desc.num_seqs
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, desc.num_kv_heads, desc.head_size,
-                 desc.block_size)
-    _check_ints(cu_q_lens, (S + 1,), "cu_q_lens")
-    _check_ints(block_tables, (S, desc.max_blocks_per_seq), "block_tables")
-    _check_ints(seq_lens, (S,), "seq_lens")
-    for t in (q, out):
-        if t.shape != (q.shape[0], desc.num_heads, desc.head_size) or dtype_code(t) != desc.dtype \
-                or not t.is_contiguous():
-            raise TLError(ERR_INVALID_ARGUMENT, f"q / out {tuple(t.shape)} {t.dtype}: contiguous [total_q, "
-                          f"{desc.num_heads}, {desc.head_size}] of the descriptor's type")
-    _on_gpu(q, out, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens)
-    check(lib.tl_chunked_prefill_scaled(
-        ctypes.byref(desc), _ptr(out), _ptr(q), _ptr(cu_q_lens), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
-        _ptr(v_scales), _ptr(block_tables), _ptr(seq_lens), q.shape[0], max_q_len, _stream(stream)))
+    S, n_kv, D = desc.num_seqs, desc.num_kv_heads, desc.head_size
+    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size)
+    _check(cu_q_lens, (S + 1,), I32, "cu_q_lens")
+    _check(block_tables, (S, desc.max_blocks_per_seq), I32, "block_tables")
+    _check(seq_lens, (S,), I32, "seq_lens")
+    rows = (q.shape[0], desc.num_heads, D)
+    _check(q, rows, desc.dtype, "q")
+    _check(out, rows, desc.dtype, "out")
+    at = _on_gpu(out, q, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens)
+    check(lib.tl_chunked_prefill_scaled(ctypes.byref(desc), *at, q.shape[0], max_q_len, _stream(stream)))
 
 
 # ---------------------------------------------------------------------------
