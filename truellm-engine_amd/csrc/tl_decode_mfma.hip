@@ -59,13 +59,13 @@ __device__ __forceinline__ bool item_of(const Params& p, bool final, bool late_e
 // (item_of's late_exit), for grids that fit the GPU in one round, where the
 // launch is a chain of round trips (length, table, K/V, partials) and the
 // few loads of an exiting workgroup cost less than a round trip.
-template <Kind KV, Kind QK, Kind PO, int NW, bool FINAL, int BS, bool LATE = false>
+template <Kind KV, Kind QK, Kind PO, int NW, bool FINAL, int BS, bool LATE = false, int ITERS = 0>
 __global__ __launch_bounds__(NW * kWave) void fp8_decode_kernel(Params p) {
   __shared__ __attribute__((aligned(16))) float s_acc[NW * mw::kHeads * mw::kHead];
   __shared__ float s_m[NW * mw::kHeads], s_l[NW * mw::kHeads];
   Item w;
   if (!item_of(p, FINAL, LATE, w)) return;
-  mw::decode_workgroup<KV, QK, PO, NW, FINAL, BS, LATE>(p, w.seq, w.kvh, w.hs, w.part, w.t0, w.t1, s_acc,
+  mw::decode_workgroup<KV, QK, PO, NW, FINAL, BS, LATE, ITERS>(p, w.seq, w.kvh, w.hs, w.part, w.t0, w.t1, s_acc,
                                                                s_m, s_l, w.len);
 }
 
@@ -124,8 +124,8 @@ template <Kind KV, Kind QK, int NW, bool FINAL, int BS, Kind PO_SPLIT = Kind::F3
 void launch_kernel(const Params& p, unsigned grid, hipStream_t stream) {
   constexpr Kind PO = FINAL ? QK : PO_SPLIT;
   if constexpr (is_fp8<KV>())
-    hipLaunchKernelGGL((fp8_decode_kernel<KV, QK, PO, NW, FINAL, BS, LATE>), dim3(grid), dim3(NW * kWave), 0, stream,
-                       p);
+    hipLaunchKernelGGL((fp8_decode_kernel<KV, QK, PO, NW, FINAL, BS, LATE, ITERS>), dim3(grid), dim3(NW * kWave), 0,
+                       stream, p);
   else
     hipLaunchKernelGGL((mfma2_decode_kernel<KV, PO, NW, FINAL, BS, LATE, ITERS>), dim3(grid), dim3(NW * kWave), 0,
                        stream, p);
@@ -136,10 +136,10 @@ void launch_kernel(const Params& p, unsigned grid, hipStream_t stream) {
 template <Kind KV, Kind QK, int NW, int BS, Kind PO_SPLIT>
 void launch_late(const Params& p, unsigned grid, hipStream_t stream) {
   const int step = NW * mw::tokens_per_iteration<KV>();
-  if (!is_fp8<KV>() && p.partition_tokens <= step)
+  if (p.partition_tokens <= step)
     launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 1>(p, grid, stream);
   else if (!is_fp8<KV>() && p.partition_tokens <= 2 * step)
-    launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 2>(p, grid, stream);
+    launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, is_fp8<KV>() ? 0 : 2>(p, grid, stream);
   else
     launch_kernel<KV, QK, NW, false, BS, PO_SPLIT, true, 0>(p, grid, stream);
 }

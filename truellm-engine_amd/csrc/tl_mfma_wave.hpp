@@ -286,11 +286,10 @@ __device__ __forceinline__ void scale_tokens(V& s, float x) {
 // 32/8 heads, bf16: 87.5 us, 6.33 TB/s (FP8, 256 bytes of a token and
 // head in place of 264, 82.9 us, 6.48; with products of scales that are not
 // folded, a divide and branches in the block's pick 88.4).
-template <Kind KV, Kind QK, int BS, class Flush = NoFlush>
+template <Kind KV, Kind QK, int BS, class Flush = NoFlush, int ITERS = 0>
 __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int hs, int first_it, int t1,
                                           int step, const Flush& flush = Flush(), int len = 0x7fffffff) {
   static_assert(BS >= 8 && (BS & (BS - 1)) == 0, "block size: a power of two >= 8");
-  t1 = min(t1, len);
   constexpr int TPI = 64, RB = BS;           // tokens per iteration; bytes per head-dim row of a block
   constexpr bool kSplitRun = BS == 8;        // a lane's 16-token V run spans two blocks
   constexpr bool kScaled = KV == Kind::FP8S;
@@ -298,50 +297,6 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
   constexpr int NB = blocks_per_iteration<BS, TPI>();
   const int lane = threadIdx.x % kWave;
   const int m = lane & 15, kg = lane >> 4;
-
-  // ---- q of head column m in MFMA order: slot (s, e) = dim 32 s + 4 e + kg ----
-  const int gi = hs * kHeads + m;
-  const bool hv = gi < p.group;
-  const int head = hv ? head_of(p, kvh, gi) : 0;
-  const uint16_t* qrow = (const uint16_t*)p.q + ((int64_t)seq * p.num_heads + head) * kHead;
-  // the loads under one condition, used after it: loads under a condition
-  // of their own were each a branch with a wait, 32 round trips in a row
-  uint16_t qh[32] = {};
-  if (hv) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qh[8 * s + e] = qrow[32 * s + 4 * e + kg];
-  }
-  float qf[32];
-  float qmax = 0.f;
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint16_t bits = qh[8 * s + e];
-      const float v = QK == Kind::BF16 ? bf16_to_f32(bits) : f16_to_f32(bits);
-      qf[8 * s + e] = v;
-      qmax = fmaxf(qmax, fabsf(v));
-    }
-  int sh = 0;
-  if constexpr (QK == Kind::BF16) {
-    qmax = max_kg(qmax);
-    if (qmax > 0.f && qmax < INFINITY) {
-      int ex;
-      frexpf(qmax, &ex);
-      sh = 15 - ex;
-    }
-  }
-  u4v qb[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    h8 v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (_Float16)ldexpf(qf[8 * s + e], sh);
-    qb[s] = __builtin_bit_cast(u4v, v);
-  }
-  const float qk_scale = p.qk_scale * ldexpf(1.f, -sh);
 
   State st;
   st.init();
@@ -415,9 +370,30 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
   float ks = 0.f, vs = 0.f;
   if constexpr (kScaled) st.no_unit();
 
+  // The prologue in the order of its round trips: the sequence's length
+  // (t1, len) and the table entries in flight together, then q and the first
+  // K/V, and q is brought into its order while they fly.
   int it = first_it;
-  Blocks<NB> cur = table_blocks<NB, BS>(p, table, it, t1);
-  Blocks<NB> nxt = table_blocks<NB, BS>(p, table, it + step, t1);
+  Blocks<NB> cur_raw = table_raw<NB, BS>(p, table, it);
+  Blocks<NB> nxt_raw = ITERS == 1 ? cur_raw : table_raw<NB, BS>(p, table, it + step);
+  // (opaque, or the reads are moved behind the length's)
+#pragma unroll
+  for (int i = 0; i < NB; ++i) asm volatile("" : "+s"(cur_raw.e[i]), "+s"(nxt_raw.e[i]));
+  t1 = min(t1, len);
+  if (it >= t1) return st;
+  Blocks<NB> cur = table_check<NB, BS>(p, cur_raw, it, t1);
+  Blocks<NB> nxt = table_check<NB, BS>(p, nxt_raw, it + step, t1);
+
+  // ---- q of head column m: dims 32 kg + 8 i .. + 7 ----
+  const int gi = hs * kHeads + m;
+  const bool hv = gi < p.group;
+  const int head = hv ? head_of(p, kvh, gi) : 0;
+  const uint16_t* qrow = (const uint16_t*)p.q + ((int64_t)seq * p.num_heads + head) * kHead;
+  u32x4 ql[4] = {};
+  if (hv) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) __builtin_memcpy(&ql[i], qrow + 32 * kg + 8 * i, 16);   // aligned to its elements
+  }
   uint32_t kw[32];
   u32x4 vr[8];
   {
@@ -430,20 +406,65 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
     }
     __builtin_amdgcn_sched_barrier(0);
     load_v(vr, v_at(cur, ib, vb), v_at(cur, ib, vb2));
+    __builtin_amdgcn_sched_barrier(0);
   }
 
-#pragma unroll 1
-  for (; it < t1; it += step) {
-    if constexpr (Flush::kActive) {
-      if (it != first_it && it % flush.part_tokens == 0) {   // a partition ends: its partials out, state afresh
-        flush(st, it / flush.part_tokens - 1);
-        st.init();
-        if constexpr (kScaled) st.no_unit();
+  // ---- q in MFMA order: slot (s, e) = dim 32 s + 4 e + kg ----
+  // Opaque until here, or q is waited for under its condition.  Lane row kg
+  // has the dims of step s = kg; the 4 x 4 dwords (pairs of e) of the lane
+  // rows are transposed.
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ql[i].x), "+v"(ql[i].y), "+v"(ql[i].z), "+v"(ql[i].w));
+  u4v qb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = 0x05040100u, hi = 0x07060302u;
+    // dims 8 i + k and 8 i + 4 + k of this lane row's step
+    const uint32_t x0 = __builtin_amdgcn_perm(ql[i].z, ql[i].x, lo), x1 = __builtin_amdgcn_perm(ql[i].z, ql[i].x, hi);
+    const uint32_t x2 = __builtin_amdgcn_perm(ql[i].w, ql[i].y, lo), x3 = __builtin_amdgcn_perm(ql[i].w, ql[i].y, hi);
+    const auto a02 = __builtin_amdgcn_permlane32_swap(x0, x2, false, false);
+    const auto a13 = __builtin_amdgcn_permlane32_swap(x1, x3, false, false);
+    const auto y01 = __builtin_amdgcn_permlane16_swap((unsigned)a02[0], (unsigned)a13[0], false, false);
+    const auto y23 = __builtin_amdgcn_permlane16_swap((unsigned)a02[1], (unsigned)a13[1], false, false);
+    qb[0][i] = y01[0];
+    qb[1][i] = y01[1];
+    qb[2][i] = y23[0];
+    qb[3][i] = y23[1];
+  }
+  float qk_scale = p.qk_scale;
+  if constexpr (QK == Kind::BF16) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = qb[s][i];
+        top = max(top, max(w << 16 & 0x7fffffffu, w & 0x7fff0000u));
       }
+    const float qmax = max_kg(__builtin_bit_cast(float, top));
+    int sh = 0;
+    if (qmax > 0.f && qmax < INFINITY) {
+      int ex;
+      frexpf(qmax, &ex);
+      sh = 15 - ex;
     }
-    const Blocks<NB> nn = table_blocks<NB, BS>(p, table, it + 2 * step, t1);
-    const int ib_next = in_block_bytes<BS, TPI, 1>(it + step);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = qb[s][i];
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        h2 v;
+        v[0] = (_Float16)ldexpf(__builtin_bit_cast(float, w << 16), sh);
+        v[1] = (_Float16)ldexpf(__builtin_bit_cast(float, w & 0xffff0000u), sh);
+        qb[s][i] = __builtin_bit_cast(uint32_t, v);
+      }
+    qk_scale *= ldexpf(1.f, -sh);
+  }
 
+  // One iteration at token it of table entries c; with reload, the K/V of
+  // entries ld (in-block offset ib_ld) are then loaded.
+  auto iterate = [&](const Blocks<NB>& c, const Blocks<NB>& ld, int ib_ld, bool reload) {
     // ---- q.k: 4 tiles (token i of each quad) x 4 MFMA steps ----
     f4 s[4];
 #pragma unroll
@@ -477,16 +498,16 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
     // the next iteration's loads are issued whether or not it exists (a
     // missing one reads block 0): under a condition the compiler would
     // wait for them, too, before this iteration's V is used
-    load_k(kw, kbase0 + ib_next + (int64_t)max(pick(nxt, kb), 0) * pool_stride);
+    if (reload) load_k(kw, kbase0 + ib_ld + (int64_t)max(pick(ld, kb), 0) * pool_stride);
 
     // ---- softmax: lane (m, kg) owns head m, iteration tokens 16 kg + 4 r + i ----
-    const int ph_v = pick(cur, vb);
+    const int ph_v = pick(c, vb);
     int n_ok;
     uint32_t keep = 0xffffu;   // block size 8: the run's tokens that exist (bit t: token 16 kg + t)
     if constexpr (kSplitRun) {
       n_ok = min(max(t1 - (it + 16 * kg), 0), 16);
       keep = (n_ok >= 16 ? 0xffffu : ((1u << n_ok) - 1u)) & (ph_v < 0 ? 0xff00u : 0xffffu) &
-             (pick(cur, vb2) < 0 ? 0x00ffu : 0xffffu);
+             (pick(c, vb2) < 0 ? 0x00ffu : 0xffffu);
     } else {
       n_ok = ph_v < 0 ? 0 : min(max(t1 - (it + 16 * kg), 0), 16);
     }
@@ -513,11 +534,11 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
       }
     if constexpr (kScaled) {
       // the lane's own token: past the end or in a hole its scale may be anything
-      const float v_own = scale_block(cur) >= 0 && it + lane < t1 ? vs : 0.f;
+      const float v_own = scale_block(c) >= 0 && it + lane < t1 ? vs : 0.f;
       st.raise_unit(v_own);
       scale_tokens(pw, v_own * st.inv_unit);
       // the next iteration's, after this one's last use of the registers
-      load_scales(nxt, ib_next, ks, vs);
+      if (reload) load_scales(ld, ib_ld, ks, vs);
     }
     // P^T operands: MFMA h takes tokens 8 h .. 8 h + 7 = (r = 2 h, 2 h + 1) x (i = 0 .. 3).
     // Where out is f16 (kLow) the rest that rounding a weight to f16 leaves
@@ -561,9 +582,27 @@ __device__ __forceinline__ State fp8_wave(const Params& p, int seq, int kvh, int
         st.o[dt] = mma<Kind::F16>(a[4], a[5], a[6], a[7], pl[1], st.o[dt]);
       }
     }
-    load_v(vr, v_at(nxt, ib_next, vb), v_at(nxt, ib_next, vb2));
-    cur = nxt;
-    nxt = nn;
+    if (reload) load_v(vr, v_at(ld, ib_ld, vb), v_at(ld, ib_ld, vb2));
+  };
+
+  if constexpr (ITERS == 1) {
+    static_assert(!Flush::kActive, "partition flushes stream whole partitions");
+    iterate(cur, cur, 0, false);
+  } else {
+#pragma unroll 1
+    for (; it < t1; it += step) {
+      if constexpr (Flush::kActive) {
+        if (it != first_it && it % flush.part_tokens == 0) {   // a partition ends: its partials out, state afresh
+          flush(st, it / flush.part_tokens - 1);
+          st.init();
+          if constexpr (kScaled) st.no_unit();
+        }
+      }
+      const Blocks<NB> nn = table_blocks<NB, BS>(p, table, it + 2 * step, t1);
+      iterate(cur, nxt, in_block_bytes<BS, TPI, 1>(it + step), true);
+      cur = nxt;
+      nxt = nn;
+    }
   }
   return st;
 }
@@ -795,7 +834,7 @@ template <Kind KV, Kind QK, int BS, class Flush = NoFlush, int ITERS = 0>
 __device__ __forceinline__ State run_wave(const Params& p, int seq, int kvh, int hs, int first_it, int t1,
                                           int step, const Flush& flush = Flush(), int len = 0x7fffffff) {
   if constexpr (is_fp8<KV>())
-    return fp8_wave<KV, QK, BS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
+    return fp8_wave<KV, QK, BS, Flush, ITERS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
   else
     return mfma2_wave<KV, BS, Flush, ITERS>(p, seq, kvh, hs, first_it, t1, step, flush, len);
 }
