@@ -292,31 +292,33 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _on_gpu(*tensors):
-    """The tensors' pointers (None: null); refuses one that is not on the current device, whose streams and kernels
-    would not reach it."""
-    here = _torch().cuda.current_device() if tensors[0].is_cuda else -2
-    at = []
-    for t in tensors:
-        if t is None:
-            at.append(None)
-        elif t.get_device() == here:
-            at.append(t.data_ptr())
-        else:
-            raise TLError(ERR_INVALID_ARGUMENT, f"a tensor on {t.device}, not on the current GPU")
-    return at
+def _here(t):
+    """The current device, whose streams and kernels reach only its own tensors; -2 (none has it) where t is not on a
+    GPU.  Read, as the stream below, as torch's own launchers read it: the public calls cost as much as a launch."""
+    if not t.is_cuda:
+        return -2
+    torch = _torch()
+    get = getattr(torch._C, "_cuda_getDevice", None)
+    return torch.cuda.current_device() if get is None else get()
 
 
-def _stream(stream=None):
-    """The stream's handle; without one, that of the current device's current stream (read as torch's own launchers
-    read it: the stream object costs as much as a launch)."""
+def _at(t, shape, dtype, here, what):
+    """The pointer of a contiguous tensor of this shape and tl_dtype (or I32) on device `here`."""
+    if t.shape != shape or t.dtype is not _DTYPE_OF[dtype] or not t.is_contiguous() or t.get_device() != here:
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype} on {t.device}: contiguous "
+                      f"{tuple(shape)} of {_DTYPE_OF[dtype]} on the current GPU")
+    return t.data_ptr()
+
+
+def _stream(stream=None, here=None):
+    """The stream's handle; without one, that of the current stream of device `here` (the current one)."""
     if stream is not None:
         return stream.cuda_stream
     torch = _torch()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is None or not torch.cuda.is_initialized():
         return torch.cuda.current_stream().cuda_stream
-    return raw(torch.cuda.current_device())
+    return raw(torch.cuda.current_device() if here is None else here)
 
 
 # ---------------------------------------------------------------------------
@@ -413,19 +415,15 @@ def fused_add_rms_norm(out, residual, x, weight, eps, stream=None):
 
 def _norm_fp8(fn, out, scales, residual, x, weight, eps, group_size, stream):
     """An FP8 norm's call (residual: () without one); the library cannot see the tensors' sizes."""
-    shape, dtype = x.shape, x.dtype
+    shape, code = x.shape, dtype_code(x)
     T, H = shape
-    want = (T, H // group_size) if group_size > 0 else (T,)
-    if not (out.shape == shape and out.element_size() == 1 and scales.shape == want and weight.shape == (H,)
-            and weight.dtype == dtype and scales.dtype is _DTYPE_OF[F32] and x.is_contiguous() and out.is_contiguous()
-            and scales.is_contiguous() and weight.is_contiguous()):
-        raise TLError(ERR_INVALID_ARGUMENT, f"x {tuple(shape)} {dtype}: out {tuple(out.shape)} {out.dtype}, "
-                      f"scales {tuple(scales.shape)} {scales.dtype} (fp32 {want}), weight {tuple(weight.shape)} "
-                      f"{weight.dtype}, all contiguous")
-    for r in residual:
-        if r is None or not (r.shape == shape and r.dtype == dtype and r.is_contiguous()):
-            raise TLError(ERR_INVALID_ARGUMENT, f"residual {r if r is None else (tuple(r.shape), r.dtype)}")
-    check(fn(*_on_gpu(out, scales, *residual, x, weight), T, H, group_size, eps, dtype_code(x), _stream(stream)))
+    here = _here(x)
+    if out.shape != shape or out.element_size() != 1 or not out.is_contiguous() or out.get_device() != here:
+        raise TLError(ERR_INVALID_ARGUMENT, f"out {tuple(out.shape)} {out.dtype} on {out.device}: contiguous "
+                      f"{tuple(shape)} of one byte on the current GPU")
+    check(fn(out.data_ptr(), _at(scales, (T, H // group_size) if group_size > 0 else (T,), F32, here, "scales"),
+             *[_at(r, shape, code, here, "residual") for r in residual], _at(x, shape, code, here, "x"),
+             _at(weight, (H,), code, here, "weight"), T, H, group_size, eps, code, _stream(stream, here)))
 
 
 def rms_norm_fp8(out, scales, x, weight, eps, group_size=0, stream=None):
@@ -436,6 +434,8 @@ def rms_norm_fp8(out, scales, x, weight, eps, group_size=0, stream=None):
 
 def fused_add_rms_norm_fp8(out, scales, residual, x, weight, eps, group_size=0, stream=None):
     """rms_norm_fp8 of residual + x, which replaces residual (in its dtype)."""
+    if residual is None:
+        raise TLError(ERR_INVALID_ARGUMENT, "no residual")
     _norm_fp8(lib.tl_fused_add_rms_norm_fp8, out, scales, (residual,), x, weight, eps, group_size, stream)
 
 
@@ -520,23 +520,18 @@ def _token_stride(t, T, heads, head_size, dtype, what):
     return st[0] if T > 1 else 0
 
 
-def _check(t, shape, dtype, what):
-    """A contiguous tensor of this shape and tl_dtype (or I32)."""
-    if t.shape != shape or t.dtype is not _DTYPE_OF[dtype] or not t.is_contiguous():
-        raise TLError(ERR_INVALID_ARGUMENT, f"{what} {tuple(t.shape)} {t.dtype}: contiguous {tuple(shape)} of "
-                      f"{_DTYPE_OF[dtype]}")
+def _rows_at(t, here, what):
+    if t.get_device() != here:
+        raise TLError(ERR_INVALID_ARGUMENT, f"{what} on {t.device}, not on the current GPU")
+    return t.data_ptr()
 
 
-def _check_pools(k_cache, v_cache, k_scales, v_scales, kv_dtype, num_blocks, heads, head_size, block_size):
+def _pools_at(k_cache, v_cache, k_scales, v_scales, kv_dtype, num_blocks, heads, head_size, block_size, here):
     """Pools [N, n_kv, D, bs] of one type, and their scales (None: none) fp32 [N, n_kv, bs]."""
-    shape = (num_blocks, heads, head_size, block_size)
-    _check(k_cache, shape, kv_dtype, "k_cache")
-    _check(v_cache, shape, kv_dtype, "v_cache")
-    shape = (num_blocks, heads, block_size)
-    if k_scales is not None:
-        _check(k_scales, shape, F32, "k_scales")
-    if v_scales is not None:
-        _check(v_scales, shape, F32, "v_scales")
+    shape, per_row = (num_blocks, heads, head_size, block_size), (num_blocks, heads, block_size)
+    return (_at(k_cache, shape, kv_dtype, here, "k_cache"), _at(v_cache, shape, kv_dtype, here, "v_cache"),
+            None if k_scales is None else _at(k_scales, per_row, F32, here, "k_scales"),
+            None if v_scales is None else _at(v_scales, per_row, F32, here, "v_scales"))
 
 
 def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_cache, slot_mapping, positions, cos_table,
@@ -545,37 +540,33 @@ def rope_axes_reshape_and_cache(desc: RopeAxesDesc, q, key, value, k_cache, v_ca
     key/value into the pools; FP8 pools (uint8) take k_scales / v_scales fp32 [N, n_kv, bs], one scale per token and
     head.  q, q_out, key and value may be slices of a wider tensor (their token strides are read)."""
     T, H, n_kv, D, dtype = key.shape[0], desc.num_heads, desc.num_kv_heads, desc.head_size, desc.dtype
-    q_out = q if q_out is None else q_out
+    here = _here(key)
     sq = so = 0
+    q_at = to_at = None
     if H:
-        sq = _token_stride(q, T, H, D, dtype, "q")
-        so = sq if q_out is q else _token_stride(q_out, T, H, D, dtype, "q_out")
-    else:
-        q = q_out = None
+        q_out = q if q_out is None else q_out
+        sq, q_at = _token_stride(q, T, H, D, dtype, "q"), _rows_at(q, here, "q")
+        so, to_at = (sq, q_at) if q_out is q else (_token_stride(q_out, T, H, D, dtype, "q_out"),
+                                                   _rows_at(q_out, here, "q_out"))
     sk, sv = _token_stride(key, T, n_kv, D, dtype, "key"), _token_stride(value, T, n_kv, D, dtype, "value")
-    _check_pools(k_cache, v_cache, k_scales, v_scales, desc.kv_dtype, desc.num_blocks, n_kv, D, desc.block_size)
-    _check(slot_mapping, (T,), I32, "slot_mapping")
-    _check(positions, (desc.num_axes, T), I32, "positions")
     table = (desc.max_positions, D // 2)
-    _check(cos_table, table, F32, "cos_table")
-    _check(sin_table, table, F32, "sin_table")
-    key_at, *at = _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, positions, cos_table, sin_table,
-                          q, q_out)
-    check(lib.tl_rope_axes_reshape_and_cache(ctypes.byref(desc), at[9], at[10], key_at, *at[:9], T, sq, so, sk, sv,
-                                             _stream(stream)))
+    check(lib.tl_rope_axes_reshape_and_cache(
+        ctypes.byref(desc), q_at, to_at, _rows_at(key, here, "key"), _rows_at(value, here, "value"),
+        *_pools_at(k_cache, v_cache, k_scales, v_scales, desc.kv_dtype, desc.num_blocks, n_kv, D, desc.block_size, here),
+        _at(slot_mapping, (T,), I32, here, "slot_mapping"), _at(positions, (desc.num_axes, T), I32, here, "positions"),
+        _at(cos_table, table, F32, here, "cos_table"), _at(sin_table, table, F32, here, "sin_table"), T, sq, so, sk, sv,
+        _stream(stream, here)))
 
 
 def reshape_and_cache_fp8_scaled(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, stream=None):
     """reshape_and_cache_fp8 with a scale for each token and head, found here: k_scales / v_scales fp32
     [N, n_kv, bs]."""
     T, n_kv, D = key.shape
-    BS, N, code = k_cache.shape[3], k_cache.shape[0], dtype_code(key)
-    _check(key, key.shape, code, "key")
-    _check(value, key.shape, code, "value")
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, N, n_kv, D, BS)
-    _check(slot_mapping, (T,), I32, "slot_mapping")
-    key_at, value_at, *at = _on_gpu(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
-    check(lib.tl_reshape_and_cache_fp8_scaled(key_at, value_at, code, *at, T, n_kv, D, BS, N, _stream(stream)))
+    BS, N, code, here = k_cache.shape[3], k_cache.shape[0], dtype_code(key), _here(key)
+    check(lib.tl_reshape_and_cache_fp8_scaled(
+        _at(key, key.shape, code, here, "key"), _at(value, key.shape, code, here, "value"), code,
+        *_pools_at(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, N, n_kv, D, BS, here),
+        _at(slot_mapping, (T,), I32, here, "slot_mapping"), T, n_kv, D, BS, N, _stream(stream, here)))
 
 
 def _block_bytes(pool):
@@ -652,20 +643,19 @@ def paged_attention_decode(desc: DecodeDesc, out, q, k_cache, v_cache, block_tab
 def paged_attention_decode_scaled(desc: DecodeDesc, out, q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
                                   max_context_len, workspace=None, stream=None):
     """paged_attention_decode over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
-    S, n_kv, D = desc.num_seqs, desc.num_kv_heads, desc.head_size
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size)
-    _check(block_tables, (S, desc.max_blocks_per_seq), I32, "block_tables")
-    _check(seq_lens, (S,), I32, "seq_lens")
+    S, n_kv, D, here = desc.num_seqs, desc.num_kv_heads, desc.head_size, _here(q)
     rows = (S, desc.num_heads, D)
-    _check(q, rows, desc.q_dtype, "q")
-    _check(out, rows, desc.q_dtype, "out")
-    ws_bytes = 0
+    ws, ws_bytes = None, 0
     if workspace is not None:
-        if not workspace.is_contiguous():
-            raise TLError(ERR_INVALID_ARGUMENT, f"workspace strides {workspace.stride()}: contiguous")
-        ws_bytes = workspace.numel() * workspace.element_size()
-    *at, ws = _on_gpu(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, workspace)
-    check(lib.tl_paged_attention_decode_scaled(ctypes.byref(desc), *at, max_context_len, ws, ws_bytes, _stream(stream)))
+        if not workspace.is_contiguous() or workspace.get_device() != here:
+            raise TLError(ERR_INVALID_ARGUMENT, f"workspace of strides {workspace.stride()} on {workspace.device}: "
+                          f"contiguous, on the current GPU")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(lib.tl_paged_attention_decode_scaled(
+        ctypes.byref(desc), _at(out, rows, desc.q_dtype, here, "out"), _at(q, rows, desc.q_dtype, here, "q"),
+        *_pools_at(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size, here),
+        _at(block_tables, (S, desc.max_blocks_per_seq), I32, here, "block_tables"),
+        _at(seq_lens, (S,), I32, here, "seq_lens"), max_context_len, ws, ws_bytes, _stream(stream, here)))
 
 
 NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -857,16 +847,14 @@ def chunked_prefill(desc, out, q, cu_q_lens, k_cache, v_cache, block_tables, seq
 def chunked_prefill_scaled(desc, out, q, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens,
                            max_q_len, stream=None):
     """chunked_prefill over FP8 pools (uint8) with a scale for each token and kv head, fp32 [N, n_kv, bs]."""
-    S, n_kv, D = desc.num_seqs, desc.num_kv_heads, desc.head_size
-    _check_pools(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size)
-    _check(cu_q_lens, (S + 1,), I32, "cu_q_lens")
-    _check(block_tables, (S, desc.max_blocks_per_seq), I32, "block_tables")
-    _check(seq_lens, (S,), I32, "seq_lens")
+    S, n_kv, D, here = desc.num_seqs, desc.num_kv_heads, desc.head_size, _here(q)
     rows = (q.shape[0], desc.num_heads, D)
-    _check(q, rows, desc.dtype, "q")
-    _check(out, rows, desc.dtype, "out")
-    at = _on_gpu(out, q, cu_q_lens, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens)
-    check(lib.tl_chunked_prefill_scaled(ctypes.byref(desc), *at, q.shape[0], max_q_len, _stream(stream)))
+    check(lib.tl_chunked_prefill_scaled(
+        ctypes.byref(desc), _at(out, rows, desc.dtype, here, "out"), _at(q, rows, desc.dtype, here, "q"),
+        _at(cu_q_lens, (S + 1,), I32, here, "cu_q_lens"),
+        *_pools_at(k_cache, v_cache, k_scales, v_scales, FP8_E4M3, desc.num_blocks, n_kv, D, desc.block_size, here),
+        _at(block_tables, (S, desc.max_blocks_per_seq), I32, here, "block_tables"),
+        _at(seq_lens, (S,), I32, here, "seq_lens"), rows[0], max_q_len, _stream(stream, here)))
 
 
 # ---------------------------------------------------------------------------
