@@ -69,7 +69,8 @@ __global__ __launch_bounds__(NW * kWave) void fp8_decode_kernel(Params p) {
                                                                s_m, s_l, w.len);
 }
 
-// ITERS: 1 or 2 when no wavefront has more iterations (mw::mfma2_wave).
+// ITERS: 1 or 2 (2-byte KV only) when no wavefront has more iterations
+// (mw::mfma2_wave).
 template <Kind KV, Kind PO, int NW, bool FINAL, int BS, bool LATE = false, int ITERS = 0>
 __global__ __launch_bounds__(NW * kWave) void mfma2_decode_kernel(Params p) {
   __shared__ __attribute__((aligned(16))) float s_acc[NW * mw::kHeads * mw::kHead];
@@ -186,11 +187,14 @@ int launch_typed(const DecodeLaunch& a) {
     p.stash_floats = 4 * stash * (int)sizeof(float) <= 64 * 1024 ? stash : 0;
     hipLaunchKernelGGL((wave_partition_kernel<KV, QK, BS>), dim3(items * ((runs + 3) / 4)), dim3(4 * kWave),
                        4 * p.stash_floats * sizeof(float), a.stream, p);
-  } else if (items * P <= 128) {
+  } else if (items * P <= 128 && p.partition_tokens > 4 * mw::tokens_per_iteration<KV>()) {
     // a grid of at most half the CUs (the engine's one-sequence call inside
     // the v2 scratch: 8 partitions x 8 kv heads): 8 wavefronts per
     // workgroup (two per SIMD: the wavefront keeps its 256 registers), so
-    // that each streams two of a 512-token partition's iterations
+    // that each streams two of a 512-token partition's iterations.  A
+    // partition of at most 4 iterations has none for the other four: 758
+    // tokens in 128-token partitions, 64/8 heads, bf16, 12.6 us with 8 and
+    // 10.4 with 4; FP8, 256-token partitions, 9.4 either way
     if (f16_parts) {
       if constexpr (KV == Kind::F16) launch_late<KV, QK, 8, BS, Kind::F16>(p, items * P, a.stream);
     } else {
