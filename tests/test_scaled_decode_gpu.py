@@ -193,3 +193,15 @@ def test_scaled_decode_replayed_graph():
             assert torch.equal(out, want)
         else:
             check(p, q, out)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[3000], [5, 100, 700]])
+def test_scaled_decode_of_a_q_aligned_to_its_elements(dt, lens):
+    p = Pools(lens, 8, 16, seed=4)
+    q = queries(len(lens), 32, dt)
+    odd = torch.empty(q.numel() + 9, dtype=dt, device="cuda")
+    for shift in (1, 2, 5):
+        view = odd[shift:shift + q.numel()].view(q.shape)
+        view.copy_(q)
+        check(p, view, decode(p, view), what=f"shift {shift}")
