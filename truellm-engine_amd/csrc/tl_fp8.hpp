@@ -29,6 +29,12 @@ __device__ __forceinline__ Fp8Scale fp8_scale_of(uint32_t amax_bits) {
   const float s = __builtin_bit_cast(float, amax_bits) / 448.0f;
   return s >= 1.17549435e-38f ? Fp8Scale{s, 1.0f / s} : Fp8Scale{0.f, 0.f};
 }
+// Elements times the inverse of their own row's scale, which is a few parts in
+// 2^23 above 448 at most and so rounds to it: not saturated.
+__device__ __forceinline__ uint32_t pack4_fp8_found(float a, float b, float c, float d) {
+  const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, (int)w, true);
+}
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
 // A lane's bits of another lane of its row of 16 (a DPP control of tl_device.hpp).
