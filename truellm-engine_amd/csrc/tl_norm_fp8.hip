@@ -120,8 +120,8 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_fp8_rows_kernel(NormFp8
     const Fp8Scale s = fp8_scale_of(m);
     if (i0 % a.group == 0) a.scales[row * (a.hidden / a.group) + i0 / a.group] = s.scale;
     *reinterpret_cast<uint2*>(a.out + base + i0) =
-        make_uint2(pack4_fp8(v[c][0] * s.inv, v[c][1] * s.inv, v[c][2] * s.inv, v[c][3] * s.inv),
-                   pack4_fp8(v[c][4] * s.inv, v[c][5] * s.inv, v[c][6] * s.inv, v[c][7] * s.inv));
+        make_uint2(pack4_fp8_found(v[c][0] * s.inv, v[c][1] * s.inv, v[c][2] * s.inv, v[c][3] * s.inv),
+                   pack4_fp8_found(v[c][4] * s.inv, v[c][5] * s.inv, v[c][6] * s.inv, v[c][7] * s.inv));
   }
   if (a.group != 0) return;
   const Fp8Scale s = fp8_scale_of(TPR == kWave ? lanes_umax<kWave>(top) : block_umax(top, s_max));
@@ -131,8 +131,8 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_fp8_rows_kernel(NormFp8
     const int i0 = (c * TPR + t) * 8;
     if (i0 >= a.hidden) break;
     *reinterpret_cast<uint2*>(a.out + base + i0) =
-        make_uint2(pack4_fp8(v[c][0] * s.inv, v[c][1] * s.inv, v[c][2] * s.inv, v[c][3] * s.inv),
-                   pack4_fp8(v[c][4] * s.inv, v[c][5] * s.inv, v[c][6] * s.inv, v[c][7] * s.inv));
+        make_uint2(pack4_fp8_found(v[c][0] * s.inv, v[c][1] * s.inv, v[c][2] * s.inv, v[c][3] * s.inv),
+                   pack4_fp8_found(v[c][4] * s.inv, v[c][5] * s.inv, v[c][6] * s.inv, v[c][7] * s.inv));
   }
 }
 
