@@ -304,3 +304,27 @@ def test_rope_axes_replayed_graph_and_another_stream(kv, T, slots):
         again()
         graph.replay()
         same()
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_the_scale_of_every_magnitude(dt):
+    """A row of one magnitude for each positive finite value: scale a / 448 to the bit, as fp32 divides, and the code
+    of 448 (0x7E) or, negative, of -448; below 448 x 2^-126 the scale 0 and zeros."""
+    n = 0x7C00 if dt == torch.float16 else 0x7F80
+    a = torch.arange(n, dtype=torch.int16).view(dt)
+    want = a.float() / 448
+    want[want < 2.0 ** -126] = 0
+    key = a.view(n, 1, 1).expand(n, 1, 128).contiguous().cuda()
+    BS, N = 16, (n + 15) // 16
+    k, v = (torch.full((N, 1, 128, BS), 0x55, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((N, 1, BS), -1.0, device="cuda") for _ in range(2))
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    for part in (slice(0, n), slice(5, 300)):                # tiles, and a step
+        tla.reshape_and_cache_fp8_scaled(key[part], -key[part], k, v, ks, vs, slots[part])
+        torch.cuda.synchronize()
+        for scales, codes, sign in ((ks, k, 0), (vs, v, 0x80)):
+            assert torch.equal(scales.view(-1)[part].cpu(), want[part])
+            rows = codes.permute(0, 3, 1, 2).reshape(-1, 128)[part].cpu()
+            live = want[part] > 0
+            assert (rows[live] == 0x7E | sign).all() and ((rows[~live] & 0x7F) == 0).all()
+        ks.fill_(-1.0), vs.fill_(-1.0), k.fill_(0x55), v.fill_(0x55)

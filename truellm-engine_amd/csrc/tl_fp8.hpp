@@ -26,8 +26,16 @@ struct Fp8Scale {
 };
 __device__ __forceinline__ Fp8Scale fp8_scale_of(uint32_t amax_bits) {
   if (amax_bits >= 0x7f800000u) return {__builtin_bit_cast(float, 0x7fc00000u), __builtin_bit_cast(float, 0x7fc00000u)};
-  const float s = __builtin_bit_cast(float, amax_bits) / 448.0f;
-  return s >= 1.17549435e-38f ? Fp8Scale{s, 1.0f / s} : Fp8Scale{0.f, 0.f};
+  // The quotient by the constant, corrected by its exact remainder: the same
+  // number as a / 448 for every a with a normal quotient; and the reciprocal
+  // with one Newton step, within 2^-24 (checked on the CPU over whole binades
+  // and the threshold's).  A division is about ten instructions, these are
+  // three and four.
+  constexpr float kInv = 1.0f / 448.0f;
+  const float a = __builtin_bit_cast(float, amax_bits), q = a * kInv;
+  const float s = __builtin_fmaf(__builtin_fmaf(-q, 448.0f, a), kInv, q);
+  const float r = __builtin_amdgcn_rcpf(s), inv = __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r);
+  return s >= 1.17549435e-38f ? Fp8Scale{s, inv} : Fp8Scale{0.f, 0.f};
 }
 // Elements times the inverse of their own row's scale, which is a few parts in
 // 2^23 above 448 at most and so rounds to it: not saturated.
