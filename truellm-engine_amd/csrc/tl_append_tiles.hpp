@@ -257,9 +257,9 @@ __device__ __forceinline__ void rotate_q_tile(const TileAppend& a, int wg) {
 // tables' entries of one pair of one token, which all of the token's heads take
 // from LDS, so that pairs whose axes differ cost one read each, not one for
 // every head; the heads' first elements are on their way meanwhile.  Bound by
-// HBM: 4055 tokens of 64/8 heads into scaled FP8 pools 36.4 us, 4.4 TB/s (at
-// 36.9 us, with 4 tokens to a workgroup, of whose 8 units a thread 4 are in flight, 43.5; as
-// rotate_q_tile, the tables read by every thread, 46.0).
+// HBM: 4055 tokens of 64/8 heads into scaled FP8 pools 36.4 us, 4.4 TB/s (36.9
+// when it came in; with 4 tokens to a workgroup, of whose 8 units a thread 4 are
+// in flight, 43.5; as rotate_q_tile, the tables read by every thread, 46.0).
 inline __host__ __device__ int axes_q_tokens(int num_heads, int head_size) {
   const int fit = kTileThreads / (head_size / 2), units = num_heads * (head_size / 16);
   return max(1, min(fit, kTileThreads / units));
